@@ -222,7 +222,8 @@ def _norm(s):
     pad = -width % group
     ug = torch.nn.functional.pad(u, (0, pad)).view(rows, -1, group)
     top = ug.abs().amax(-1)
-    to = torch.where(top > 1e-30, TOP[c["out"]] / top, 0.0)
+    # a division of tensors rounds once (a number over a tensor is a reciprocal and a product)
+    to = torch.where(top > 1e-30, torch.full_like(top, TOP[c["out"]]).div(top), 0.0)
     q = (ug * to.unsqueeze(-1)).view(rows, -1)[:, :width]
     q = q.round().to(torch.int8) if c["out"] == "i8" else q.to(torch.float8_e4m3fn)
     inv = (h.double().square().mean(-1, keepdim=True) + EPS).rsqrt()
