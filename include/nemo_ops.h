@@ -7,8 +7,8 @@
  * reference's per-kernel `createRun` / `encode` pairs stand
  * (src/webgpu/ops.ts, src/webgpu/quant-matmul.ts): same inputs, same
  * outputs, packed valid-token rows instead of padded [batch x sequence] rows.
- * Every call launches on the legacy default stream and synchronises before it
- * returns; errors follow nemo.h.
+ * Unless its comment says otherwise, a call launches on the legacy default
+ * stream and synchronises before it returns; errors follow nemo.h.
  */
 #ifndef NEMO_OPS_H
 #define NEMO_OPS_H
@@ -127,6 +127,132 @@ int nemo_op_qmatmul(int fmt, const void* d_packed, const void* d_x, int m, int n
  * src/gguf/quantization.ts:19-74 rounded to f16 as quant-matmul.ts:106 does.
  * Synchronises. */
 int nemo_op_qmatmul_image_decode(int fmt, const void* d_image, int n, int k, void* d_w16);
+
+/* --- Layer operators beside the fixed-shape encoder -------------------------
+ * Operators of a transformer layer for other shapes and types than the
+ * encoder's own: residual RMSNorm with an 8-bit output, rotary embedding,
+ * 4-bit group-quantised matrix-vector product, windowed attention. No
+ * counterpart in the reference.
+ *
+ * They are asynchronous: each enqueues its kernel on `stream` (a cudaStream_t,
+ * NULL = legacy default stream) and returns. They allocate nothing, keep
+ * nothing between calls, use no workspace and can be captured into CUDA
+ * graphs; calls on different streams are independent of one another. Every
+ * buffer is device memory of one device, which need not be the current one;
+ * `stream` belongs to that device. Leading dimensions (ld*) count elements
+ * between the starts of consecutive rows. Zero rows, tokens or requests is a
+ * valid call that does nothing. Inputs and outputs do not overlap unless an
+ * entry says so. Results do not depend on the launch: the same call on the
+ * same inputs gives the same bits. */
+#define NEMO_DTYPE_F16 0
+#define NEMO_DTYPE_BF16 1
+#define NEMO_DTYPE_F32 2
+#define NEMO_DTYPE_E4M3 3 /* 8-bit float, 4 exponent and 3 mantissa bits, largest value 448 */
+#define NEMO_DTYPE_I8 4
+
+/* Residual RMSNorm with an 8-bit output. For each row of `width` columns, in
+ * f32:
+ *   s = x + residual (s = x with d_residual NULL); d_sum = s rounded to dtype;
+ *   u = s * w; for each group of `group` columns top = max|u| and
+ *   q = round(u * (Q / top)), scale = top / Q / sqrt(mean(s^2) + eps),
+ * Q = 448 for NEMO_DTYPE_E4M3 and 127 for NEMO_DTYPE_I8, both rounded to
+ * nearest even, so that q * scale is the normalised row. dtype (x, residual,
+ * sum) is F16 or BF16, d_w f32 [width]. group is 32, 64 or 128 (the last group
+ * of a row may be shorter), or 0 for one scale per row; d_scales is f32
+ * [rows x ceil(width / group)]. d_sum is NULL exactly when d_residual is; it
+ * may be d_x or d_residual themselves (with the same ld). A group whose top is
+ * at most 1e-30 has codes 0; one that holds an infinity or a NaN has codes 0
+ * and a NaN scale. width <= 32768. Rows of 16-byte multiples with 16-byte
+ * aligned buffers (8-byte for d_q) are read and written as vectors; others
+ * work, slower. */
+int nemo_op_rmsnorm_q8(int dtype, const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, const void* d_w,
+                       int rows, int width, float eps, void* d_sum, int64_t lds, int out_dtype, int group, void* d_q,
+                       int64_t ldq, void* d_scales, void* stream);
+
+/* Rotary embedding of q and k: element pair i of the first rotary_dim columns
+ * of each head turns by t = position * inv_freq[i],
+ *   (a, b) -> magnitude * (a cos t - b sin t, a sin t + b cos t),
+ * computed in f32 with t reduced in 64 bits (positions up to 2^31 - 1 keep
+ * their angle); columns from rotary_dim to head_dim are copied. layout
+ * NEMO_ROPE_PAIRS pairs columns (2i, 2i + 1), NEMO_ROPE_HALVES (i,
+ * i + rotary_dim / 2). q rows hold q_heads heads of head_dim columns, k rows
+ * k_heads; heads follow one another, rows are ldq / ldk apart (a column range
+ * of a QKV buffer is fine). d_k may be NULL with k_heads 0. d_inv_freq f64
+ * [rotary_dim / 2], d_positions int32 [tokens]. d_qo may be d_q with ldqo ==
+ * ldq, and d_ko d_k (in place). dtype F16 or BF16; rotary_dim even and at most
+ * head_dim; head_dim <= 512. */
+#define NEMO_ROPE_PAIRS 0
+#define NEMO_ROPE_HALVES 1
+int nemo_op_rope_apply(int dtype, int layout, const void* d_q, int64_t ldq, int q_heads, const void* d_k, int64_t ldk,
+                       int k_heads, int head_dim, int rotary_dim, const void* d_inv_freq, float magnitude,
+                       const void* d_positions, int tokens, void* d_qo, int64_t ldqo, void* d_ko, int64_t ldko,
+                       void* stream);
+
+/* Inverse frequencies for nemo_op_rope_apply, on the host: out [rotary_dim / 2]
+ * f64 and *magnitude. With f_i = theta^(-2i / rotary_dim):
+ *   NEMO_ROPE_PLAIN   f_i
+ *   NEMO_ROPE_LINEAR  f_i / factor
+ *   NEMO_ROPE_NTK     theta' = theta * factor^(r / (r - 2)), r = rotary_dim >= 4
+ *   NEMO_ROPE_YARN    f_i / factor blended into f_i over the pairs that turn
+ *                     between `slow` (1) and `fast` (32) times in
+ *                     original_context positions (boundaries rounded outwards
+ *                     to whole pairs, as in nemo_rope_table), *magnitude =
+ *                     0.1 ln(factor) + 1
+ *   NEMO_ROPE_RAMP    the same blend over the number of turns itself
+ *                     (slow 1, fast 4): f_i / factor below `slow` turns, f_i
+ *                     above `fast`, magnitude 1
+ * *magnitude is 1 for the others. factor >= 1; original_context, slow and fast
+ * (0 < slow < fast) are read by the last two only. */
+#define NEMO_ROPE_PLAIN 0
+#define NEMO_ROPE_LINEAR 1
+#define NEMO_ROPE_NTK 2
+#define NEMO_ROPE_YARN 3
+#define NEMO_ROPE_RAMP 4
+int nemo_rope_inv_freq(int scaling, double theta, int rotary_dim, double factor, double original_context, double slow,
+                       double fast, double* out, float* magnitude);
+
+/* Matrix-vector products with 4-bit weights and group scales, for up to 16
+ * rows of x at once:
+ *   y[m x n] = x[m x k] . W[n x k]^T,  W[r][c] = scale[r][c / group] * (q[r][c] - zero[r][c / group]).
+ * d_w4 holds two columns per byte, the even one in the low four bits
+ * ([n x k / 2] bytes, 16-byte aligned); d_scales [n x k / group] of scale_dtype
+ * (F16 or BF16); d_zeros packs the zero points the same way ([n x
+ * ceil(k / group / 2)] bytes), NULL = 8 everywhere. group is 32, 64 or 128 and
+ * divides k. x is F16, BF16, E4M3 or I8; 8-bit codes take d_x_scales f32
+ * [m x ceil(k / x_group)], x_group 32, 64 or 128, or >= k for one scale per
+ * row (as nemo_op_rmsnorm_q8 writes them, where group 0 is x_group >= k);
+ * 16-bit x takes NULL. y is F16, BF16 or F32. Products q - zero are exact and
+ * sums are f32; y is rounded once. m > 16 is refused: nemo_op_qmatmul serves
+ * batches. d_x and ldx need the alignment of one element only. */
+int nemo_op_w4_matvec(int x_dtype, const void* d_x, int64_t ldx, const void* d_x_scales, int x_group, const void* d_w4,
+                      int scale_dtype, const void* d_scales, const void* d_zeros, int group, int m, int n, int k,
+                      int y_dtype, void* d_y, int64_t ldy, void* stream);
+
+/* Grouped-query attention with a sliding window and first tokens that stay
+ * visible, for prompts, whole documents and single tokens against a cache.
+ * Request b has the query rows d_q_off[b] .. d_q_off[b + 1] - 1 (int32
+ * [batch + 1], ascending) and the key rows d_k_start[b] .. + d_k_len[b] - 1
+ * (int32 [batch] each), so keys may be packed like the queries or lie in a
+ * cache with room behind them. Its queries are the last ones of its keys:
+ * query i has position p = i + key length - query length, and sees key j iff
+ *   j < key length  and  (right < 0 or j <= p + right)
+ *   and  (left < 0 or j >= p - left or j < sinks).
+ * right 0 is causal, right < 0 with left < 0 bidirectional. A query that sees
+ * no key gets zeros. Scores are q . k * scale with an f32 softmax, weights are
+ * rounded to dtype for the product with v, which sums in f32. Infinities and
+ * NaN in keys or values that a query does not see do not reach its row.
+ * dtype F16 or BF16; head_dim 64 or 128; q_heads a multiple of kv_heads; heads
+ * follow one another within a row; buffers 16-byte aligned, leading dimensions
+ * multiples of 8. q_rows, k_rows: rows of the buffers. max_q: the longest
+ * query length (rows past it are not written). max_k: about the longest key
+ * length, which only steers the split of the work. Rows of d_out that no
+ * request covers stay as they are. d_err is a zeroed 4-byte device word that
+ * becomes nonzero if a bounded wait gave up. */
+int nemo_op_attention_window(int dtype, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v,
+                             int64_t ldv, int q_heads, int kv_heads, int head_dim, const void* d_q_off,
+                             const void* d_k_start, const void* d_k_len, int batch, int q_rows, int k_rows, int max_q,
+                             int max_k, int left, int right, int sinks, float scale, void* d_out, int64_t ldo,
+                             void* d_err, void* stream);
 
 /* Routing of the head-parallel path (no reference counterpart; the index
  * functions its QKV GEMM and attention epilogues use, exported for layout

@@ -1,0 +1,202 @@
+// Launchers of the layer operators of nemo_ops.h (rmsnorm_q8, rope_apply,
+// w4_matvec, attention_window) and the device helpers they share. Arguments
+// are checked by the C entry points (layer_ops.cu) before a launcher runs.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace nemo {
+
+enum DType { kDtF16 = 0, kDtBF16 = 1, kDtF32 = 2, kDtE4M3 = 3, kDtI8 = 4 };
+
+struct NormQ8Args {
+  const void* x;
+  const void* residual;
+  const float* w;
+  void* sum;
+  void* q;
+  float* scales;
+  int64_t ldx, ldr, lds, ldq;
+  int rows, width, group, groups;
+  float eps;
+  int dtype, out_dtype;
+};
+cudaError_t launch_rmsnorm_q8(const NormQ8Args& a, cudaStream_t s);
+
+struct RopeApplyArgs {
+  const void* q;
+  const void* k;
+  void* qo;
+  void* ko;
+  const double* inv_freq;
+  const int* positions;
+  int64_t ldq, ldk, ldqo, ldko;
+  int q_heads, k_heads, head_dim, rotary_dim, tokens;
+  float magnitude;
+  int dtype, layout;
+};
+cudaError_t launch_rope_apply(const RopeApplyArgs& a, cudaStream_t s);
+
+struct W4Args {
+  const void* x;
+  const float* x_scales;
+  const uint8_t* w;
+  const uint16_t* scales;
+  const uint8_t* zeros;
+  void* y;
+  int64_t ldx, ldy;
+  int x_dtype, scale_dtype, y_dtype;
+  int x_group, group, m, n, k;
+};
+cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s);
+
+struct AttnWindowArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const int* q_off;
+  const int* k_start;
+  const int* k_len;
+  uint32_t* err;
+  int64_t ldq, ldk, ldv, ldo;
+  int q_heads, kv_heads, head_dim, batch, q_rows, k_rows, max_q, max_k;
+  int left, right, sinks;  // left, right < 0: unbounded
+  float scale;
+  int dtype;
+};
+cudaError_t launch_attention_window(const AttnWindowArgs& a, cudaStream_t s);
+
+// Launches with programmatic dependent launch: the grid may start while the
+// previous kernel of the stream drains, which hides the launch latency. Every
+// kernel launched this way waits (dev::pdl_wait) before its first access to
+// global memory, so stream order holds for all data. cluster: CTAs per cluster
+// along x or y (0 = none).
+template <typename... P, typename... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, dim3 cluster,
+                              A... args) {
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cluster.x * cluster.y > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster.x;
+    attr[1].val.clusterDim.y = cluster.y;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+namespace dev {
+
+// Two 16-bit values of a 32-bit word as f32, and back (round to nearest even).
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<T>(w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+
+// D[16 x 8] += A[16 x 16] . B[16 x 8], 16-bit inputs, f32 accumulation, in one warp.
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                  uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16-byte asynchronous copy to shared memory; bytes 0 writes zeros instead.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes = 16) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace dev
+}  // namespace nemo

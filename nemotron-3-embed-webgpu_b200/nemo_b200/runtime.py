@@ -51,6 +51,7 @@ def load_library() -> ctypes.CDLL:
         raise ImportError(f"{LIB_PATH} is missing: build it with `make -C {os.path.dirname(LIB_PATH)}`")
     L = ctypes.CDLL(LIB_PATH)
     P, S, I, U32 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint32
+    I64, F32, F64 = ctypes.c_int64, ctypes.c_float, ctypes.c_double
     sig = {
         "nemo_model_load": (I, [P, S, P, I, ctypes.POINTER(P)]),
         "nemo_model_destroy": (None, [P]),
@@ -90,6 +91,12 @@ def load_library() -> ctypes.CDLL:
         "nemo_op_qmatmul_enqueue": (I, [I, P, P, I, I, I, P, P, P]),
         "nemo_op_qmatmul_image_decode": (I, [I, P, I, I, P]),
         "nemo_op_qmatmul": (I, [I, P, P, I, I, I, P]),
+        "nemo_op_rmsnorm_q8": (I, [I, P, I64, P, I64, P, I, I, F32, P, I64, I, I, P, I64, P, P]),
+        "nemo_op_rope_apply": (I, [I, I, P, I64, I, P, I64, I, I, I, P, F32, P, I, P, I64, P, I64, P]),
+        "nemo_rope_inv_freq": (I, [I, F64, I, F64, F64, F64, F64, P, ctypes.POINTER(F32)]),
+        "nemo_op_w4_matvec": (I, [I, P, I64, P, I, P, I, P, P, I, I, I, I, I, P, I64, P]),
+        "nemo_op_attention_window": (I, [I, P, I64, P, I64, P, I64, I, I, I, P, P, P, I, I, I, I, I, I, I, I, F32, P,
+                                         I64, P, P]),
         "nemo_hp_qkv_route": (I, [I, P, P, P]),
         "nemo_hp_row_owner": (I, [I, I, I, P]),
         "nemo_tokenizer_load": (I, [P, S, ctypes.POINTER(P)]),

@@ -1,0 +1,442 @@
+"""The layer operators of include/nemo_ops.h on the GPU against 64-bit forms (layer_ops_ref.py), where they can go
+wrong: sizes around the tiles, strides, groups, windows that leave a row empty, garbage where nothing may look, streams
+and graphs, and one layer's run of them together."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import layer_ops_ref as ref
+from layer_ops_ref import BF16, E4M3, F16, F32, I8, TORCH
+from nemo_b200.runtime import NemoError, check, load_library
+
+pytestmark = pytest.mark.gpu
+
+TYPES = pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+
+
+@pytest.fixture
+def gen():
+    g = torch.Generator(device="cuda")
+    g.manual_seed(77)
+    return g
+
+
+def normal(gen, *shape, dt=F32):
+    return torch.randn(shape, generator=gen, device="cuda").to(TORCH[dt])
+
+
+# --- rmsnorm_q8 ------------------------------------------------------------------
+
+@TYPES
+@pytest.mark.parametrize("out", [E4M3, I8], ids=["e4m3", "i8"])
+@pytest.mark.parametrize("rows,width", [(1, 2048), (3, 1), (5, 7), (300, 64), (33, 129), (9, 5120), (2, 12296),
+                                        (2, 32768), (700, 1000)])
+def test_rmsnorm_q8(gen, dt, out, rows, width):
+    x = normal(gen, rows, width, dt=dt) * 3
+    w = 1 + 0.2 * normal(gen, width)
+    r = normal(gen, rows, width, dt=dt)
+    for group in (0, 32, 64, 128):
+        for res in (None, r):
+            got = ref.rmsnorm_q8(x, res, w, 1e-5, out, group)
+            ref.check_rmsnorm_q8(x, res, w, 1e-5, out, group, got)
+
+
+def test_rmsnorm_q8_strides_and_in_place(gen):
+    rows, width = 37, 256
+    for ld in (width + 3, width + 8):  # rows that are not, and that are, 16 bytes apart
+        x, r = normal(gen, rows, ld, dt=F16), normal(gen, rows, ld, dt=F16)
+        w = normal(gen, width)
+        q = torch.full((rows, ld), 5, dtype=torch.int8, device="cuda")
+        want = ref.rmsnorm_q8(x[:, :width].contiguous(), r[:, :width].contiguous(), w, 1e-5, I8, 64)
+        before = x.clone()
+        total, _, scales = ref.rmsnorm_q8(x[:, :width], r[:, :width], w, 1e-5, I8, 64, total=x[:, :width],
+                                          q=q[:, :width])
+        assert torch.equal(total, want[0]) and torch.equal(q[:, :width], want[1]) and torch.equal(scales, want[2])
+        assert torch.equal(x[:, width:], before[:, width:]) and (q[:, width:] == 5).all()  # the gaps stay
+
+
+def test_rmsnorm_q8_zeros_infinities_and_nan(gen):
+    x = normal(gen, 4, 256, dt=BF16)
+    w = torch.ones(256, device="cuda")
+    x[0] = 0
+    x[1, 130] = float("nan")
+    x[2, 10] = float("inf")
+    x[3, 64:128] = 0
+    _, q, s = ref.rmsnorm_q8(x, None, w, 1e-5, E4M3, 64)
+    q = q.view(torch.uint8)
+    assert (q[0] == 0).all() and (s[0] == 0).all()
+    assert torch.isnan(s[1]).all() and (q[1, 128:192] == 0).all()
+    assert torch.isnan(s[2, 0]) and (s[2, 1:] == 0).all() and (q[2, :64] == 0).all()
+    assert (q[3, 64:128] == 0).all() and s[3, 1] == 0 and (s[3, [0, 2, 3]] > 0).all()
+    _, q, s = ref.rmsnorm_q8(torch.zeros_like(x), None, w, 0.0, I8, 0)  # 0 / 0 without eps
+    assert (q == 0).all()
+
+
+# --- rope ------------------------------------------------------------------------
+
+def inv_freq(scaling, theta, rotary, *rest):
+    out, mag = np.zeros(rotary // 2), ctypes.c_float()
+    check(load_library().nemo_rope_inv_freq(scaling, theta, rotary, *rest, out.ctypes.data_as(ctypes.c_void_p),
+                                            ctypes.byref(mag)))
+    return torch.from_numpy(out).cuda(), mag.value
+
+
+@TYPES
+@pytest.mark.parametrize("layout", [0, 1], ids=["pairs", "halves"])
+@pytest.mark.parametrize("tokens,hq,hk,d,rotary", [
+    (1, 24, 8, 128, 128), (5, 3, 1, 128, 64), (77, 4, 4, 64, 64), (3, 2, 1, 80, 40), (2, 5, 0, 96, 2), (4, 1, 1, 6, 4),
+    (3, 2, 2, 256, 256), (2, 1, 1, 512, 512), (2, 1, 1, 511, 510), (600, 24, 8, 128, 32)])
+def test_rope_apply(gen, dt, layout, tokens, hq, hk, d, rotary):
+    q = normal(gen, tokens, hq, d, dt=dt)
+    k = normal(gen, tokens, hk, d, dt=dt) if hk else None
+    freq, mag = inv_freq(3, 1e6, rotary, 16.0, 4096.0, 1.0, 32.0)
+    pos = torch.randint(0, 40000, (tokens,), generator=gen, device="cuda", dtype=torch.int32)
+    qo, ko = ref.rope_apply(q, k, freq, mag, pos, rotary, layout)
+    ref.check_rope(q, freq, mag, pos, rotary, layout, qo)
+    if hk:
+        ref.check_rope(k, freq, mag, pos, rotary, layout, ko)
+
+
+@pytest.mark.parametrize("layout", [0, 1], ids=["pairs", "halves"])
+@pytest.mark.parametrize("pad", [8, 3])
+def test_rope_apply_in_a_qkv_buffer_in_place(gen, layout, pad):
+    tokens, hq, hk, d, rotary = 19, 6, 2, 64, 32
+    ld = (hq + 2 * hk) * d + pad
+    buf = normal(gen, tokens, ld, dt=F16)
+    before = buf.clone()
+    q = torch.as_strided(buf, (tokens, hq, d), (ld, d, 1))
+    k = torch.as_strided(buf, (tokens, hk, d), (ld, d, 1), hq * d)
+    freq, mag = inv_freq(0, 1e4, rotary, 1.0, 0.0, 0.0, 0.0)
+    pos = torch.arange(tokens, device="cuda", dtype=torch.int32)
+    wq, wk = q.clone(), k.clone()
+    ref.rope_apply(q, k, freq, mag, pos, rotary, layout, qo=q, ko=k)
+    ref.check_rope(wq, freq, mag, pos, rotary, layout, q)
+    ref.check_rope(wk, freq, mag, pos, rotary, layout, k)
+    assert torch.equal(buf[:, (hq + hk) * d:], before[:, (hq + hk) * d:])
+
+
+def test_rope_apply_far_positions_keep_their_angle(gen):
+    q = normal(gen, 4, 1, 64, dt=F16)
+    freq, mag = inv_freq(0, 1e6, 64, 1.0, 0.0, 0.0, 0.0)
+    pos = torch.tensor([0, 1, 999999, 2 ** 31 - 1], device="cuda", dtype=torch.int32)
+    qo, _ = ref.rope_apply(q, None, freq, mag, pos, 64, 0)
+    ref.check_rope(q[:3], freq, mag, pos[:3], 64, 0, qo[:3])
+    # the 64-bit product of the farthest position is itself off by 2^-23 of a turn
+    t = pos[3:].double()[:, None] * freq
+    a, b = q[3:, 0, 0::2].double(), q[3:, 0, 1::2].double()
+    ref.close(qo[3:, 0, 0::2], a * torch.cos(t) - b * torch.sin(t), 2.0 ** -10 * (a.abs() + b.abs()))
+
+
+# --- w4 --------------------------------------------------------------------------
+
+def w4_inputs(gen, xt, m, n, k, group, zeros, st, x_group):
+    q = torch.randint(0, 16, (n, k), generator=gen, device="cuda")
+    z = torch.randint(0, 16, (n, k // group), generator=gen, device="cuda") if zeros else None
+    s = (0.01 * normal(gen, n, k // group)).to(TORCH[st])
+    xs = None
+    if xt in (E4M3, I8):
+        x = (normal(gen, m, k) * (100 if xt == E4M3 else 40)).clamp(-127, 127)
+        x = (x.round() if xt == I8 else x).to(TORCH[xt])
+        xs = 0.01 + 0.02 * torch.rand((m, -(-k // x_group)), generator=gen, device="cuda")
+    else:
+        x = normal(gen, m, k, dt=xt)
+    return x, xs, q, s, z
+
+
+@pytest.mark.parametrize("xt", [F16, BF16, E4M3, I8], ids=["f16", "bf16", "e4m3", "i8"])
+@pytest.mark.parametrize("group,x_group", [(128, 128), (64, 32), (32, 10 ** 6), (128, 64), (32, 128)])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 128), (1, 2048, 2048), (2, 17, 384), (3, 100, 1024), (5, 5120, 256),
+                                   (8, 33, 2176), (9, 64, 6144), (16, 4800, 640), (16, 16, 8192), (1, 40, 20480)])
+def test_w4_matvec(gen, xt, group, x_group, m, n, k):
+    zeros, st, yt = (m + n) % 2 == 1, (F16, BF16)[m % 2], (F32, F16, BF16)[(m + k // 128) % 3]
+    x, xs, q, s, z = w4_inputs(gen, xt, m, n, k, group, zeros, st, x_group)
+    y = ref.w4_matvec(x, xs, x_group, ref.pack4(q), s, ref.pack4(z) if zeros else None, group, n, yt)
+    ref.check_w4(x, xs, x_group, q, s, z, group, y, yt)
+
+
+def test_w4_matvec_strides_and_odd_addresses(gen):
+    m, n, k = 6, 50, 512
+    x, _, q, s, z = w4_inputs(gen, F16, m, n, k, 64, True, F16, k)
+    wide = torch.full((m, k + 5), float("nan"), dtype=torch.float16, device="cuda")
+    wide[:, 1:k + 1] = x  # rows two bytes past a 16-byte boundary and odd bytes apart
+    y = torch.full((m, n + 7), 9.0, device="cuda")
+    ref.w4_matvec(wide[:, 1:k + 1], None, 0, ref.pack4(q), s, ref.pack4(z), 64, n, F32, y=y[:, :n])
+    ref.check_w4(x, None, k, q, s, z, 64, y[:, :n], F32)
+    assert (y[:, n:] == 9.0).all()
+    bytes_x = torch.randint(-127, 128, (m, k + 3), generator=gen, device="cuda", dtype=torch.int8)
+    xs = torch.rand((m, 4), generator=gen, device="cuda")
+    y = ref.w4_matvec(bytes_x[:, 1:k + 1], xs, 128, ref.pack4(q), s, ref.pack4(z), 64, n, F32)
+    ref.check_w4(bytes_x[:, 1:k + 1], xs, 128, q, s, z, 64, y, F32)
+
+
+def test_w4_matvec_rows_do_not_mix(gen):
+    """A NaN in one row of x and an infinite scale in one row of W stay in theirs."""
+    m, n, k = 4, 64, 256
+    x, _, q, s, _ = w4_inputs(gen, F16, m, n, k, 128, False, F16, k)
+    x[2, 5] = float("nan")
+    s[7, 0] = float("inf")
+    y = ref.w4_matvec(x, None, 0, ref.pack4(q), s, None, 128, n, F32)
+    bad = ~torch.isfinite(y)
+    want = torch.zeros_like(bad)
+    want[2], want[:, 7] = True, True
+    assert torch.equal(bad, want)
+
+
+# --- attention -------------------------------------------------------------------
+
+def packed(gen, dt, qs, ks, hq, hk, d):
+    q = normal(gen, sum(qs), hq, d, dt=dt)
+    k, v = normal(gen, sum(ks), hk, d, dt=dt), normal(gen, sum(ks), hk, d, dt=dt)
+    q_off = [0] + np.cumsum(qs).tolist()
+    return q, k, v, q_off, [0] + np.cumsum(ks).tolist()[:-1], list(ks)
+
+
+WINDOWS = [(-1, -1, 0), (-1, 0, 0), (0, 0, 0), (5, 0, 3), (40, 17, 1), (200, 0, 130), (3, 300, 0), (-1, 6, 2),
+           (2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1)]
+
+
+@TYPES
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", WINDOWS, ids=lambda w: "l%d_r%d_s%d" % w)
+@pytest.mark.parametrize("qs,ks", [([1], [1]), ([1, 1, 1], [1, 700, 33]), ([3], [3]), ([17, 0, 2, 40], [17, 9, 64, 40]),
+                                   ([130, 1], [130, 300]), ([300, 257], [300, 600]), ([20, 4], [7, 0])],
+                         ids=["1", "tokens", "3", "ragged", "130", "long", "fewer_keys"])
+def test_attention_window(gen, dt, d, window, qs, ks):
+    hq, hk = (6, 2) if d == 128 else (5, 1)
+    args = packed(gen, dt, qs, ks, hq, hk, d)
+    got = ref.attention(*args, *window)
+    ref.check_attention(*args, *window, got)
+
+
+@pytest.mark.parametrize("hq,hk", [(1, 1), (8, 8), (24, 8), (32, 2), (40, 1)])
+def test_attention_window_head_layouts(gen, hq, hk):
+    for qs, ks in (([2, 1], [900, 5000]), ([150], [333])):
+        args = packed(gen, F16, qs, ks, hq, hk, 128)
+        got = ref.attention(*args, 257, 0, 4)
+        ref.check_attention(*args, 257, 0, 4, got)
+
+
+def test_attention_window_rows_without_keys_are_zeros(gen):
+    args = packed(gen, F16, [200, 5], [40, 0], 4, 2, 64)
+    got = ref.attention(*args, -1, 0, 0)
+    assert (got[:160] == 0).all() and (got[200:] == 0).all()
+    ref.check_attention(*args, -1, 0, 0, got)
+
+
+def test_attention_window_cache_with_room_and_untouched_rows(gen):
+    """Keys in a cache [request][capacity] whose unused rows hold NaN, inside a QKV-like row stride; rows of q and out
+    behind the last request stay as they were."""
+    cap, hq, hk, d = 700, 6, 2, 128
+    for q_len, lens in ((1, [0, 1, 333, 700]), (90, [90, 130, 333, 700])):
+        cache = torch.full((4 * cap, 3 * hk * d), float("nan"), dtype=torch.float16, device="cuda")
+        for b, n in enumerate(lens):
+            cache[b * cap:b * cap + n] = normal(gen, n, 3 * hk * d, dt=F16)
+        k = torch.as_strided(cache, (4 * cap, hk, d), (3 * hk * d, d, 1), hk * d)
+        v = torch.as_strided(cache, (4 * cap, hk, d), (3 * hk * d, d, 1), 2 * hk * d)
+        rows = 4 * q_len + 3
+        q = torch.full((rows, hq, d), float("nan"), dtype=torch.float16, device="cuda")
+        q[:4 * q_len] = normal(gen, 4 * q_len, hq, d, dt=F16)
+        q_off, start = [i * q_len for i in range(5)], [b * cap for b in range(4)]
+        for window in ((-1, 0, 0), (100, 0, 2)):
+            got = ref.attention(q, k, v, q_off, start, lens, *window)
+            assert (got[4 * q_len:] == 7.0).all()
+            ref.check_attention(q, k, v, q_off, start, lens, *window, got)
+
+
+@TYPES
+@pytest.mark.parametrize("q_len", [1, 4, 70, 300])
+def test_attention_window_garbage_in_unseen_keys(gen, dt, q_len):
+    """Infinities and NaN in keys and values reach the rows that see them, as NaN or infinity, and no other row."""
+    nk, hq, hk, d = 420, 4, 2, 64
+    args = packed(gen, dt, [q_len], [nk], hq, hk, d)
+    q, k, v = args[:3]
+    clean = [t.clone() for t in (k, v)]
+    left, sinks = 30, 2
+    at = nk - q_len + q_len // 2  # in the window of some queries where there are several
+    k[at, 0], v[at, 0, 3] = float("nan"), float("inf")
+    v[at, 1] = float("nan")
+    k[5], v[6] = float("inf"), float("nan")  # between the sinks and every window of a short query
+    got = ref.attention(*args, left, 0, sinks)
+    ok = ref.seen(q_len, nk, left, 0, sinks)
+    dirty = (ok[:, at] | ok[:, 5] | ok[:, 6]).cpu().numpy()
+    assert not torch.isfinite(got[dirty]).all(-1).any()
+    fine = ~dirty
+    want = torch.full_like(got, 0)
+    want[fine] = got[fine]
+    ref_got = ref.attention(q, *clean, *args[3:], left, 0, sinks)
+    ref.check_attention(q, *clean, *args[3:], left, 0, sinks, ref_got)
+    # clean rows agree with the run on clean keys to two roundings of the weights
+    assert torch.isfinite(got[fine]).all()
+    ref.close(got[fine], ref_got[fine].double(), 4 * ref.HALF[dt] * clean[1].abs().max().double())
+
+
+@pytest.mark.parametrize("q_len", [1, 200])
+def test_attention_window_large_scores(gen, q_len):
+    """Scores of several thousand: the largest key takes all the weight, nothing overflows."""
+    args = packed(gen, F16, [q_len], [500], 2, 1, 128)
+    args[0].mul_(30), args[1].mul_(30)
+    got = ref.attention(*args, -1, -1, 0, scale=1.0)
+    # scores reach 2^17, where an f32 sum of 128 products is good to about 2^-6: compare with the best key where it
+    # leads by more
+    s = torch.einsum("qhd,khd->hqk", args[0].double(), args[1].double().expand(-1, 2, -1))
+    top = s.topk(2, -1)
+    clear = (top.values[..., 0] - top.values[..., 1]) > 20
+    assert clear.any()
+    want = args[2][:, 0].double()[top.indices[..., 0]]
+    ref.close(got.permute(1, 0, 2)[clear], want[clear], 2.0 ** -10 * want[clear].abs() + 2.0 ** -16)
+
+
+@pytest.mark.parametrize("q_len", [1, 130])
+def test_attention_window_offsets_past_32_bits(q_len):
+    """A cache whose later rows lie more than 2^32 bytes in."""
+    rows, hk, d = 1_300_000, 8, 128
+    cache = torch.empty((rows, 2 * hk * d), dtype=torch.float16, device="cuda")
+    assert cache.numel() > 2 ** 31
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    n, start = 900, rows - 901
+    cache[start:start + n] = torch.randn((n, 2 * hk * d), generator=g, device="cuda").half()
+    k = torch.as_strided(cache, (rows, hk, d), (2 * hk * d, d, 1))
+    v = torch.as_strided(cache, (rows, hk, d), (2 * hk * d, d, 1), hk * d)
+    q = torch.randn((q_len, hk, d), generator=g, device="cuda").half()
+    got = ref.attention(q, k, v, [0, q_len], [start], [n], 300, 0, 4)
+    ref.check_attention(q, k, v, [0, q_len], [start], [n], 300, 0, 4, got)
+
+
+# --- how they are called ---------------------------------------------------------
+
+def test_repeats_streams_and_graphs_give_the_same_bits(gen):
+    x, r, w = normal(gen, 50, 2048, dt=F16), normal(gen, 50, 2048, dt=F16), normal(gen, 2048)
+    wx, xs, wq, s, z = w4_inputs(gen, E4M3, 3, 1024, 4096, 64, True, F16, 128)
+    w4, z4 = ref.pack4(wq), ref.pack4(z)
+    q, k, v = (normal(gen, n, 8, 128, dt=F16) for n in (300, 2000, 2000))
+    q1 = q[:2].contiguous()
+    offs = [torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0, 300], [0], [2000], [0, 2])]
+    pos = torch.arange(300, device="cuda", dtype=torch.int32)
+    freq, mag = inv_freq(0, 1e6, 128, 1.0, 0.0, 0.0, 0.0)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def buffers():
+        return {"sum": torch.zeros_like(x), "q8": torch.zeros((50, 2048), dtype=torch.int8, device="cuda"),
+                "sc": torch.zeros((50, 16), device="cuda"), "y": torch.zeros((3, 1024), device="cuda"),
+                "ro": torch.zeros_like(q), "at": torch.zeros_like(q), "a1": torch.zeros_like(q1)}
+
+    def all_of(b):
+        L, st = load_library(), ref.stream()
+        check(L.nemo_op_rmsnorm_q8(F16, x.data_ptr(), 2048, r.data_ptr(), 2048, w.data_ptr(), 50, 2048, 1e-5,
+                                   b["sum"].data_ptr(), 2048, I8, 128, b["q8"].data_ptr(), 2048, b["sc"].data_ptr(), st))
+        check(L.nemo_op_w4_matvec(E4M3, wx.data_ptr(), 4096, xs.data_ptr(), 128, w4.data_ptr(), F16, s.data_ptr(),
+                                  z4.data_ptr(), 64, 3, 1024, 4096, F32, b["y"].data_ptr(), 1024, st))
+        check(L.nemo_op_rope_apply(F16, 0, q.data_ptr(), 1024, 8, None, 0, 0, 128, 128, freq.data_ptr(), mag,
+                                   pos.data_ptr(), 300, b["ro"].data_ptr(), 1024, None, 0, st))
+        for qq, off, n, o in ((b["ro"], offs[0], 300, b["at"]), (q1, offs[3], 2, b["a1"])):
+            check(L.nemo_op_attention_window(F16, qq.data_ptr(), 1024, k.data_ptr(), 1024, v.data_ptr(), 1024, 8, 8,
+                                             128, off.data_ptr(), offs[1].data_ptr(), offs[2].data_ptr(), 1, n, 2000,
+                                             n, 2000, 700, 0, 4, 0.08, o.data_ptr(), 1024, err.data_ptr(), st))
+
+    want = buffers()
+    all_of(want)
+    torch.cuda.synchronize()
+    a, b = buffers(), buffers()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):  # two calls at once
+        for side, buf in zip(streams, (a, b)):
+            with torch.cuda.stream(side):
+                all_of(buf)
+    torch.cuda.synchronize()
+    graphs, bufs = [], [buffers(), buffers()]
+    for buf in bufs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            all_of(buf)
+        graphs.append(graph)
+    for side, graph in zip(streams, graphs):  # two captured runs at once
+        with torch.cuda.stream(side):
+            graph.replay()
+    torch.cuda.synchronize()
+    for got in (a, b, *bufs):
+        for name in want:
+            assert torch.equal(got[name], want[name]), name
+    assert int(err) == 0
+
+
+def test_host_memory_is_refused(gen):
+    host = np.zeros(4096, np.float16)
+    x, w = normal(gen, 1, 64, dt=F16), normal(gen, 64)
+    q, sc = torch.zeros((1, 64), dtype=torch.int8, device="cuda"), torch.zeros((1, 1), device="cuda")
+    with pytest.raises(NemoError, match="not device memory"):
+        check(load_library().nemo_op_rmsnorm_q8(F16, host.ctypes.data, 64, None, 0, w.data_ptr(), 1, 64, 1e-5, None, 0,
+                                                I8, 0, q.data_ptr(), 64, sc.data_ptr(), None))
+    _, got, _ = ref.rmsnorm_q8(x, None, w, 1e-5, I8, 0)  # and the next call is served
+    assert got.any()
+
+
+@pytest.mark.parametrize("captured", [False, True], ids=["eager", "graph"])
+def test_one_layer_step(gen, captured):
+    """The operators as a layer of a served model runs them, each checked against its 64-bit form on the inputs that
+    it had: residual norm to 8 bits, QKV projection, rotation into the cache, windowed attention, output projection."""
+    tokens, width, hq, hk, d, cap = 3, 1024, 8, 2, 128, 600
+    lens = [600, 1, 250]  # keys of each request with its new token
+    qkv_w = (hq + 2 * hk) * d
+    x, r, w = normal(gen, tokens, width, dt=BF16), normal(gen, tokens, width, dt=BF16), 1 + 0.1 * normal(gen, width)
+    pq = torch.randint(0, 16, (qkv_w, width), generator=gen, device="cuda")
+    ps = (0.02 * normal(gen, qkv_w, width // 64)).bfloat16()
+    oq = torch.randint(0, 16, (width, hq * d), generator=gen, device="cuda")
+    os_ = (0.02 * normal(gen, width, hq * d // 128)).bfloat16()
+    pw, ow = ref.pack4(pq), ref.pack4(oq)
+    cache_k, cache_v = (normal(gen, tokens * cap, hk, d, dt=BF16) for _ in range(2))
+    freq, mag = inv_freq(1, 1e6, d, 4.0, 0.0, 0.0, 0.0)
+    pos = torch.tensor([n - 1 for n in lens], dtype=torch.int32, device="cuda")
+    q_off = torch.arange(tokens + 1, dtype=torch.int32, device="cuda")
+    start = torch.arange(tokens, dtype=torch.int32, device="cuda") * cap
+    k_len = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    rows = (start + pos).long()
+    total, q8 = torch.empty_like(x), torch.empty((tokens, width), dtype=torch.float8_e4m3fn, device="cuda")
+    sc = torch.empty((tokens, width // 128), device="cuda")
+    qkv = torch.empty((tokens, qkv_w), dtype=torch.bfloat16, device="cuda")
+    turned = torch.empty((tokens, (hq + hk) * d), dtype=torch.bfloat16, device="cuda")
+    att = torch.empty((tokens, hq * d), dtype=torch.bfloat16, device="cuda")
+    y = torch.empty((tokens, width), dtype=torch.bfloat16, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def step():
+        L, st = load_library(), ref.stream()
+        check(L.nemo_op_rmsnorm_q8(BF16, x.data_ptr(), width, r.data_ptr(), width, w.data_ptr(), tokens, width, 1e-5,
+                                   total.data_ptr(), width, E4M3, 128, q8.data_ptr(), width, sc.data_ptr(), st))
+        check(L.nemo_op_w4_matvec(E4M3, q8.data_ptr(), width, sc.data_ptr(), 128, pw.data_ptr(), BF16, ps.data_ptr(),
+                                  None, 64, tokens, qkv_w, width, BF16, qkv.data_ptr(), qkv_w, st))
+        check(L.nemo_op_rope_apply(BF16, 1, qkv.data_ptr(), qkv_w, hq, qkv.data_ptr() + 2 * hq * d, qkv_w, hk, d, d,
+                                   freq.data_ptr(), mag, pos.data_ptr(), tokens, turned.data_ptr(), (hq + hk) * d,
+                                   turned.data_ptr() + 2 * hq * d, (hq + hk) * d, st))
+        cache_k[rows] = turned[:, hq * d:].view(tokens, hk, d)
+        cache_v[rows] = qkv[:, (hq + hk) * d:].view(tokens, hk, d)
+        check(L.nemo_op_attention_window(BF16, turned.data_ptr(), (hq + hk) * d, cache_k.data_ptr(), hk * d,
+                                         cache_v.data_ptr(), hk * d, hq, hk, d, q_off.data_ptr(), start.data_ptr(),
+                                         k_len.data_ptr(), tokens, tokens, tokens * cap, 1, cap, 255, 0, 4, d ** -0.5,
+                                         att.data_ptr(), hq * d, err.data_ptr(), st))
+        check(L.nemo_op_w4_matvec(BF16, att.data_ptr(), hq * d, None, 0, ow.data_ptr(), BF16, os_.data_ptr(), None,
+                                  128, tokens, width, hq * d, BF16, y.data_ptr(), width, st))
+
+    step()
+    if captured:
+        first = y.clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, first)
+    torch.cuda.synchronize()
+    ref.check_rmsnorm_q8(x, r, w, 1e-5, E4M3, 128, (total, q8, sc))
+    ref.check_w4(q8, sc, 128, pq, ps, None, 64, qkv, BF16)
+    ref.check_rope(qkv[:, :hq * d].view(tokens, hq, d), freq, mag, pos, d, 1, turned[:, :hq * d].view(tokens, hq, d))
+    ref.check_rope(qkv[:, hq * d:(hq + hk) * d].view(tokens, hk, d), freq, mag, pos, d, 1,
+                   turned[:, hq * d:].view(tokens, hk, d))
+    ref.check_attention(turned[:, :hq * d].view(tokens, hq, d), cache_k, cache_v, [0, 1, 2, 3], start.tolist(), lens,
+                        255, 0, 4, att.view(tokens, hq, d))
+    ref.check_w4(att, None, 0, oq, os_, None, 128, y, BF16)
+    assert int(err) == 0
