@@ -299,7 +299,7 @@ cudaError_t launch_rows(const AttnWindowArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_attention_window(const AttnWindowArgs& a, cudaStream_t s) {
+cudaError_t launch_attention_rows(const AttnWindowArgs& a, cudaStream_t s) {
   if (a.head_dim == 64)
     return a.dtype == kDtBF16 ? launch_rows<__nv_bfloat16, 64>(a, s) : launch_rows<__half, 64>(a, s);
   return a.dtype == kDtBF16 ? launch_rows<__nv_bfloat16, 128>(a, s) : launch_rows<__half, 128>(a, s);

@@ -1,0 +1,572 @@
+// Windowed attention of prompts and documents (nemo_op_attention_window) on the
+// 5th-generation tensor cores.
+//
+// Work is cut into units: 128 consecutive queries of one head. A block takes
+// two units that follow one another in the order (query tile, head of the kv
+// group), so that both read the same keys (two heads of one tile) or nearly
+// the same (neighbouring tiles), and every K and V tile it loads serves both.
+// For each unit and key tile of 128 keys:
+//   S = Q . K^T   (tcgen05, f32 in tensor memory)
+//   online softmax by the unit's four warps, one query row per thread
+//   P = 2^(S scale log2 e - m) rounded to the 16-bit type over the columns of S
+//   O += P . V    (tcgen05, P from tensor memory, O stays there)
+// While one unit is in its softmax the tensor cores work on the other.
+//
+// The window: a tile's keys start at the first visible key of the block, the
+// sinks in front of it have tiles of their own, and each product covers only
+// the 32-key chunks that some query of the unit sees. Within a tile each warp
+// leaves out the chunks that none of its 32 rows sees and masks only those
+// that some of them do not see whole.
+//
+// Bound: both the tensor cores and the exponential unit need 1024 cycles per
+// 128 x 128 tile at head size 128.
+//
+// Warps (320 threads, persistent, one block per SM): 0 copies Q, K and V (TMA),
+// 1 issues the products, 2-5 and 6-9 are the units' softmax. The copies and
+// first products of the next pair of units run under the last softmax and the
+// output of this one. All waits are bounded.
+#include "attention_window.cuh"
+#include "kernels.cuh"
+
+namespace nemo {
+namespace {
+
+constexpr int kTile = 128;
+constexpr int kMaxRequests = 1024;  // of one launch: their pair counts are summed in shared memory
+constexpr uint64_t kWaitNs = 20000000000ull;  // a row that is computed again key by key may hold a pair up for a while
+constexpr float kMaxSlack = 8.0f;   // the running maximum moves by more than 2^8 only: P <= 256
+
+template <int D>
+struct TilesCfg {
+  static constexpr int kHalf = kTile * 64 * 2;       // 128 rows x 64 columns, one 128-byte-swizzle block
+  static constexpr int kBlock = D / 64 * kHalf;      // 128 rows of Q, K or V
+  static constexpr int kStages = D == 64 ? 4 : 2;    // K and V tiles in flight
+  static constexpr int kThreads = 320;
+  static constexpr int kSmem = 1024 + 2 * kBlock + kStages * 2 * kBlock + 256 + (kMaxRequests + 1) * 4;
+  static constexpr uint32_t kTmemCols = 512;
+  static constexpr uint32_t kColS = 0, kColO = 256;  // S_t at 128 t, O_t at 256 + 128 t
+};
+
+// One unit of a block's pair.
+struct Unit {
+  int head, i0, rows;  // q head, first query, queries (0: no such unit)
+  int lo, hi;          // window keys that some query of the unit sees
+};
+
+// A pair of units and the key tiles it walks over: sink tiles first.
+struct Pair {
+  AttnRequest rq;
+  int kvh, sink, lo, hi, sink_tiles, tiles;
+  Unit u[2];
+  __device__ __forceinline__ Pair(const AttnWindowArgs& a, int b, int kvh_, int pair) : rq(a, b), kvh(kvh_) {
+    const int group = a.q_heads / a.kv_heads;
+    const int nq = min(rq.nq, a.max_q), p_off = rq.nk - rq.nq;
+    const int units = (nq + kTile - 1) / kTile * group;
+    lo = rq.nk, hi = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int n = pair * 2 + t;
+      u[t].i0 = n / group * kTile;
+      u[t].head = kvh * group + n % group;
+      u[t].rows = n < units ? min(kTile, nq - u[t].i0) : 0;
+      u[t].lo = u[t].hi = 0;
+      if (u[t].rows) {
+        const KeyRange r(a, u[t].i0 + p_off, u[t].i0 + u[t].rows - 1 + p_off, rq.nk);
+        u[t].lo = r.lo, u[t].hi = r.hi;
+        if (r.hi > 0) lo = min(lo, r.lo), hi = max(hi, r.hi);
+      }
+    }
+    if (lo > hi) lo = hi;
+    sink = min(a.sinks, lo);
+    sink_tiles = (sink + kTile - 1) / kTile;
+    tiles = sink_tiles + (hi - lo + kTile - 1) / kTile;
+  }
+  __device__ __forceinline__ void tile(int j, int& base, int& end) const {
+    if (j < sink_tiles) {
+      base = j * kTile, end = sink;
+    } else {
+      base = lo + (j - sink_tiles) * kTile, end = hi;
+    }
+    end = min(end, base + kTile);
+  }
+  // The chunks [c0, c1) of 32 keys of a tile that unit t needs.
+  __device__ __forceinline__ void chunks(int t, int base, int end, int sinks, int& c0, int& c1) const {
+    const int w0 = max(base, u[t].lo), w1 = min(end, u[t].hi), s1 = min(end, min(sinks, u[t].hi));
+    const bool window = w1 > w0, sinked = s1 > base;
+    c0 = sinked ? 0 : (w0 - base) >> 5;
+    const int last = max(window ? w1 : base, sinked ? s1 : base) - base;  // keys past the last needed one
+    c1 = (last + 31) >> 5;
+    if (last <= 0) c0 = c1 = 0;
+  }
+};
+
+// Pairs of units over all requests: item -> (request, kv head, pair).
+struct Items {
+  const int* before;  // items of the requests before each one, [requests + 1]
+  int batch, b;
+  __device__ __forceinline__ Items(const int* s, int n) : before(s), batch(n), b(0) {}
+  __device__ __forceinline__ Pair at(const AttnWindowArgs& a, int item) {
+    while (item >= before[b + 1]) ++b;  // items only grow
+    const int each = (before[b + 1] - before[b]) / a.kv_heads, in = item - before[b];
+    const int kvh = in / each;
+    return Pair(a, b, kvh, each - 1 - (in - kvh * each));  // a causal request's longest pairs first
+  }
+  __device__ __forceinline__ int total() const { return before[batch]; }
+};
+
+template <typename T>
+constexpr uint32_t idesc_type() {
+  return 0u;
+}
+template <>
+constexpr uint32_t idesc_type<__nv_bfloat16>() {
+  return (1u << 7) | (1u << 10);  // A and B bf16
+}
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Bits first..last of a 32-bit word (either may lie outside).
+__device__ __forceinline__ uint32_t bit_range(int first, int last) {
+  const uint32_t from = first <= 0 ? 0xffffffffu : first > 31 ? 0u : 0xffffffffu << first;
+  const uint32_t to = last >= 31 ? 0xffffffffu : last < 0 ? 0u : 0xffffffffu >> (31 - last);
+  return from & to;
+}
+
+// 4 x 4 transpose of 16-byte units over each four lanes: in, unit i of the
+// lane's row; out, unit (lane & 3) of row (lane & ~3) + i.
+__device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
+  auto swap = [&](uint4& x, uint4& y, int mask, bool up) {  // the lane with the bit set gives x, the other one y
+    uint4 s = up ? x : y;
+    s.x = __shfl_xor_sync(0xffffffffu, s.x, mask);
+    s.y = __shfl_xor_sync(0xffffffffu, s.y, mask);
+    s.z = __shfl_xor_sync(0xffffffffu, s.z, mask);
+    s.w = __shfl_xor_sync(0xffffffffu, s.w, mask);
+    (up ? x : y) = s;
+  };
+  swap(v[0], v[1], 1, lane & 1);
+  swap(v[2], v[3], 1, lane & 1);
+  swap(v[0], v[2], 2, lane & 2);
+  swap(v[1], v[3], 2, lane & 2);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(320, 1)
+    attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnWindowArgs a) {
+  using C = TilesCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_s = dev::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_s + 1023u) & ~1023u) - raw_s);
+  uint8_t* sQ = smem;
+  uint8_t* sKV = sQ + 2 * C::kBlock;  // stage s: K at 2 s blocks, V behind it
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::kStages * 2 * C::kBlock);
+  const uint32_t q_full = dev::smem_u32(bars), q_empty = q_full + 8;
+  const uint32_t s_full = q_full + 16, p_ready = s_full + 16, pv_done = p_ready + 16, mma_fin = pv_done + 16;
+  const uint32_t kv_full = mma_fin + 8, kv_empty = kv_full + 8 * C::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  int* before = reinterpret_cast<int*>(bars + 32);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 0 && lane == 0) {
+    dev::prefetch_tmap(&map_q);
+    dev::prefetch_tmap(&map_k);
+    dev::prefetch_tmap(&map_v);
+    dev::mbar_init(q_full, 1);
+    dev::mbar_init(q_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      dev::mbar_init(s_full + 8 * t, 1);
+      dev::mbar_init(p_ready + 8 * t, 128);
+      dev::mbar_init(pv_done + 8 * t, 1);
+    }
+    dev::mbar_init(mma_fin, 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      dev::mbar_init(kv_full + 8 * s, 1);
+      dev::mbar_init(kv_empty + 8 * s, 1);
+    }
+    dev::fence_mbar_init();
+  }
+  // TMEM is taken only after the previous kernel of the stream has ended, and
+  // the next one may start only once it is taken: neither can hold columns that
+  // the other waits for.
+  dev::pdl_wait();
+  if (warp == 1) {
+    dev::tmem_alloc(dev::smem_u32(tmem_slot), C::kTmemCols);
+    dev::tmem_relinquish();
+  }
+  if (warp == 2) {
+    // items of each request, summed by one warp
+    const int group = a.q_heads / a.kv_heads;
+    int sum = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      const int b = b0 + lane;
+      int n = 0;
+      if (b < a.batch) {
+        const int nq = min(AttnRequest(a, b).nq, a.max_q);
+        n = ((nq + kTile - 1) / kTile * group + 1) / 2 * a.kv_heads;
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += up;
+      }
+      if (b < a.batch) before[b + 1] = sum + n;
+      sum += __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) before[0] = 0;
+  }
+  dev::tc_fence_before();
+  __syncthreads();
+  dev::tc_fence_after();
+  dev::pdl_launch_dependents();
+  const uint32_t tmem = *tmem_slot;
+  Items items(before, a.batch);
+  const int total = items.total();
+
+  if (warp == 0) {
+    // ---- copies: the elected lane of the converged warp issues them ----
+    int n = 0, issued_q = 0;  // K/V tiles and Q pairs issued
+    bool ok = true;
+    for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
+      const Pair p = items.at(a, item);
+      if (!p.tiles) continue;
+      ok = __all_sync(0xffffffffu, dev::mbar_wait(q_empty, (issued_q & 1) ^ 1, a.err, kWaitNs));
+      if (!ok) break;
+      if (dev::elect_one()) {
+        dev::mbar_arrive_expect_tx(q_full, (p.u[1].rows ? 2 : 1) * C::kBlock);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (p.u[t].rows)
+            for (int h = 0; h < D / 64; ++h)
+              dev::tma_load_2d(dev::smem_u32(sQ + t * C::kBlock + h * C::kHalf), &map_q, p.u[t].head * D + h * 64,
+                               p.rq.q0 + p.u[t].i0, q_full);
+      }
+      __syncwarp();
+      ++issued_q;
+      for (int j = 0; j < p.tiles; ++j, ++n) {
+        const int st = n % C::kStages;
+        ok = __all_sync(0xffffffffu, dev::mbar_wait(kv_empty + 8 * st, ((n / C::kStages) & 1) ^ 1, a.err, kWaitNs));
+        if (!ok) break;
+        int base, end;
+        p.tile(j, base, end);
+        if (dev::elect_one()) {
+          const uint32_t fb = kv_full + 8 * st, dk = dev::smem_u32(sKV + st * 2 * C::kBlock), dv = dk + C::kBlock;
+          dev::mbar_arrive_expect_tx(fb, 2 * C::kBlock);
+          for (int h = 0; h < D / 64; ++h)
+            dev::tma_load_2d(dk + h * C::kHalf, &map_k, p.kvh * D + h * 64, p.rq.k0 + base, fb);
+          for (int h = 0; h < D / 64; ++h)
+            dev::tma_load_2d(dv + h * C::kHalf, &map_v, p.kvh * D + h * 64, p.rq.k0 + base, fb);
+        }
+        __syncwarp();
+      }
+    }
+    // no copy of this block is in flight when it leaves
+    if (issued_q) dev::mbar_wait(q_full, (issued_q - 1) & 1, a.err, 100000000ull);
+    for (int i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)
+      dev::mbar_wait(kv_full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.err, 100000000ull);
+  } else if (warp == 1) {
+    // ---- products. Per key tile j and unit t: O_t += P_t(j-1) . V(j-1)
+    // strictly before S_t(j), which overwrites P_t; the tensor pipe runs them
+    // in the order of issue ----
+    const uint32_t idesc_o = dev::make_idesc_f16(kTile, D) | idesc_type<T>() | (1u << 16);  // V MN-major
+    int n = 0, nq = 0;        // K/V tiles and Q pairs so far
+    int done[2] = {0, 0};     // softmax tiles of each unit whose P.V has been issued
+    bool ok = true;
+    for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
+      const Pair p = items.at(a, item);
+      if (!p.tiles) continue;
+      ok = __all_sync(0xffffffffu, dev::mbar_wait(q_full, nq & 1, a.err, kWaitNs));
+      ++nq;
+      int pend0[2], pend1[2] = {0, 0};  // chunks of the P that waits for its product with V
+      bool first[2] = {true, true};     // O_t of this pair is still empty
+      for (int j = 0; j <= p.tiles && ok; ++j) {
+        uint32_t stage = 0;
+        int base = 0, end = 0;
+        if (j < p.tiles) {
+          const int st = (n + j) % C::kStages;
+          if (!__all_sync(0xffffffffu, dev::mbar_wait(kv_full + 8 * st, ((n + j) / C::kStages) & 1, a.err, kWaitNs))) {
+            ok = false;
+            break;
+          }
+          p.tile(j, base, end);
+          stage = dev::smem_u32(sKV + st * 2 * C::kBlock);
+          const int rest = end - base;
+          if (rest & 31) {
+            // rows of V past the tile's last key, up to the end of its chunk,
+            // are no request's or another one's: weight 0, but they may hold
+            // infinities or NaN
+            uint8_t* v = sKV + st * 2 * C::kBlock + C::kBlock;
+            const int zero = ((rest + 31) & ~31) - rest;
+            for (int i = lane; i < zero * 8 * (D / 64); i += 32) {
+              const int h = i / (zero * 8), r = i % (zero * 8);
+              *reinterpret_cast<uint4*>(v + h * C::kHalf + rest * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+            }
+            dev::fence_proxy_async_smem();
+            __syncwarp();
+          }
+          dev::tc_fence_after();
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok) break;
+          if (pend1[t]) {
+            if (!__all_sync(0xffffffffu, dev::mbar_wait(p_ready + 8 * t, done[t] & 1, a.err, kWaitNs))) {
+              ok = false;
+              break;
+            }
+            ++done[t];
+            dev::tc_fence_after();
+            const uint32_t v = dev::smem_u32(sKV + ((n + j - 1) % C::kStages) * 2 * C::kBlock + C::kBlock);
+            for (int kk = pend0[t] * 2; kk < pend1[t] * 2; ++kk) {
+              if (dev::elect_one())
+                dev::tc_mma_f16_ts(tmem + C::kColO + t * kTile, tmem + C::kColS + t * kTile + kk * 8,
+                                   dev::make_sw128_desc_mn(v + kk * 2048, C::kHalf, 1024), idesc_o,
+                                   first[t] && kk == pend0[t] * 2 ? 0u : 1u);
+              __syncwarp();
+            }
+            first[t] = false;
+            if (dev::elect_one()) dev::tc_commit(pv_done + 8 * t);
+            __syncwarp();
+            pend1[t] = 0;
+          }
+          if (j == p.tiles) continue;
+          int c0, c1;
+          p.chunks(t, base, end, a.sinks, c0, c1);
+          if (c0 >= c1) continue;
+          // S_t for the keys of chunks [c0, c1), at their own columns
+          const uint32_t idesc_s = dev::make_idesc_f16(kTile, (c1 - c0) * 32) | idesc_type<T>();
+          const uint32_t q = dev::smem_u32(sQ + t * C::kBlock);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            if (dev::elect_one())
+              dev::tc_mma_f16(tmem + C::kColS + t * kTile + c0 * 32,
+                              dev::make_sw128_desc(q + (kk >> 2) * C::kHalf + (kk & 3) * 32),
+                              dev::make_sw128_desc(stage + (kk >> 2) * C::kHalf + c0 * 4096 + (kk & 3) * 32), idesc_s,
+                              kk != 0 ? 1u : 0u);
+            __syncwarp();
+          }
+          if (dev::elect_one()) dev::tc_commit(s_full + 8 * t);
+          __syncwarp();
+          pend0[t] = c0, pend1[t] = c1;
+        }
+        if (!ok) break;
+        // every product that reads tile j - 1, or the pair's Q, has been issued
+        if (j > 0 && dev::elect_one()) dev::tc_commit(kv_empty + 8 * ((n + j - 1) % C::kStages));
+        __syncwarp();
+        if (j == p.tiles - 1 && dev::elect_one()) dev::tc_commit(q_empty);
+        __syncwarp();
+      }
+      n += p.tiles;
+    }
+    if (dev::elect_one()) dev::tc_commit(mma_fin);
+    __syncwarp();
+    dev::mbar_wait(mma_fin, 0, a.err, 100000000ull);  // every product has retired before TMEM is freed
+  } else {
+    // ---- softmax of unit t: thread = query row ----
+    const int t = (warp - 2) >> 2, quarter = warp & 3;
+    const uint32_t rows_at = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t col_s = rows_at + C::kColS + t * kTile, col_o = rows_at + C::kColO + t * kTile;
+    const float scale = a.scale * 1.4426950408889634f;  // scores in log2 units
+    int count = 0;  // tiles of this unit so far, over all pairs
+    bool ok = true;
+    for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
+      const Pair p = items.at(a, item);
+      const Unit& u = p.u[t];
+      if (!u.rows) continue;
+      const int p_warp = u.i0 + quarter * 32 + p.rq.nk - p.rq.nq;
+      const RowKeys mine(a, p_warp + lane, p.rq.nk), top(a, p_warp, p.rq.nk), bottom(a, p_warp + 31, p.rq.nk);
+      float m = -INFINITY, l = 0.f;
+      int seen = 0;  // tiles of this pair
+      for (int j = 0; j < p.tiles; ++j) {
+        int base, end, c0, c1;
+        p.tile(j, base, end);
+        p.chunks(t, base, end, a.sinks, c0, c1);
+        if (c0 >= c1) continue;
+        ok = __all_sync(0xffffffffu, dev::mbar_wait(s_full + 8 * t, count & 1, a.err, kWaitNs));
+        if (!ok) break;
+        dev::tc_fence_after();
+        float s[kTile];
+        uint32_t any = 0, whole = 0;  // chunks that some row sees, that every row sees whole
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int j0 = base + c * 32, j1 = j0 + 31;
+          if (c >= c0 && c < c1 && j0 <= bottom.last && (j1 >= top.first || j0 < a.sinks)) any |= 1u << c;
+          if (j1 <= top.last && j1 < end && (j0 >= bottom.first || j1 < a.sinks)) whole |= 1u << c;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (any >> c & 1) dev::tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+        dev::tc_wait_ld();
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (!(any >> c & 1)) continue;
+          if (!(whole >> c & 1)) {
+            const int j0 = base + c * 32, last = min(mine.last, end - 1) - j0;
+            const uint32_t bits = bit_range(mine.first - j0, last) | bit_range(0, min(last, a.sinks - 1 - j0));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[c * 32 + i] = bits >> i & 1 ? s[c * 32 + i] : -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) tmax = fmaxf(tmax, fmaxf(s[c * 32 + i], s[c * 32 + i + 1]));
+        }
+        tmax *= scale;
+        // The running maximum of the warp's rows moves when some row's tile
+        // maximum is more than kMaxSlack above it; otherwise P is taken
+        // against the old one, at most 2^8, and O needs no rescaling.
+        const bool move = __any_sync(0xffffffffu, tmax > m + kMaxSlack);
+        const float mnew = move ? fmaxf(m, tmax) : m;
+        const float neg = mnew == -INFINITY ? 0.f : -mnew;  // no key seen yet: all weights 0
+        const float keep = m == -INFINITY ? 0.f : dev::exp2_approx(m - mnew);
+        float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c < c0 || c >= c1) continue;
+          uint32_t pr[16];
+          if (any >> c & 1) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float e0 = dev::exp2_approx(fmaf(s[c * 32 + i], scale, neg));
+              const float e1 = dev::exp2_approx(fmaf(s[c * 32 + i + 1], scale, neg));
+              sum0 += e0, sum1 += e1;
+              pr[i / 2] = dev::pack2<T>(e0, e1);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pr[i] = 0;
+          }
+          tmem_st_x16(col_s + c * 16, pr);
+        }
+        if (seen) {
+          // the previous tile's P.V is complete: O is stable
+          ok = __all_sync(0xffffffffu, dev::mbar_wait(pv_done + 8 * t, (count - 1) & 1, a.err, kWaitNs));
+          if (!ok) break;
+          if (move) {
+            dev::tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              dev::tmem_ld_32x32b_x32(col_o + c * 32, o);
+              dev::tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+              dev::tmem_st_32x32b_x32(col_o + c * 32, o);
+            }
+          }
+        }
+        dev::tc_wait_st();
+        l = l * keep + (sum0 + sum1);
+        m = mnew;
+        dev::tc_fence_before();
+        dev::mbar_arrive(p_ready + 8 * t);
+        ++seen;
+        ++count;
+      }
+      if (!ok) break;
+      if (seen) {
+        ok = __all_sync(0xffffffffu, dev::mbar_wait(pv_done + 8 * t, (count - 1) & 1, a.err, kWaitNs));
+        if (!ok) break;
+        dev::tc_fence_after();
+      }
+      // output: O / l, four lanes writing 64 bytes of a row at a time
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      T* out = static_cast<T*>(a.out) + (int64_t)(p.rq.q0 + u.i0 + quarter * 32) * a.ldo + u.head * D;
+      const int live = u.rows - quarter * 32;  // rows of the warp that exist
+      bool bad = false;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        if (seen) {
+          dev::tmem_ld_32x32b_x32(col_o + c * 32, r);
+          dev::tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0;
+        }
+        uint4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            y[i] = l == 0.f ? 0.f : __uint_as_float(r[k * 8 + i]) * inv;
+            bad |= !isfinite(y[i]);
+          }
+          v[k] = dev::pack8<T>(y);
+        }
+        transpose4(v, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rr = (lane & ~3) + i;
+          if (rr < live) *reinterpret_cast<uint4*>(out + (int64_t)rr * a.ldo + c * 32 + (lane & 3) * 8) = v[i];
+        }
+      }
+      if (seen) dev::tc_fence_before();  // orders the loads above before the next arrival on p_ready
+      uint32_t again = __ballot_sync(0xffffffffu, bad && lane < live);
+      for (; again; again &= again - 1)
+        attention_row<T>(a, p.rq, u.i0 + quarter * 32 + __ffs(again) - 1, u.head, 0, D);
+    }
+  }
+  dev::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    dev::tc_fence_after();
+    dev::tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+}  // namespace
+
+template <typename T, int D>
+static cudaError_t launch_tiles(AttnWindowArgs a, int sms, cudaStream_t s) {
+  using C = TilesCfg<D>;
+  auto kernel = attention_tiles_kernel<T, D>;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  CUtensorMap mq, mk, mv;
+  if (make_tmap_16bit(&mq, a.q, (uint64_t)a.q_heads * D, a.q_rows, a.ldq * 2, 64, kTile) ||
+      make_tmap_16bit(&mk, a.k, (uint64_t)a.kv_heads * D, a.k_rows, a.ldk * 2, 64, kTile) ||
+      make_tmap_16bit(&mv, a.v, (uint64_t)a.kv_heads * D, a.k_rows, a.ldv * 2, 64, kTile))
+    return cudaErrorInvalidValue;
+  const int group = a.q_heads / a.kv_heads;
+  const int64_t pairs = (((int64_t)a.max_q + kTile - 1) / kTile * group + 1) / 2 * a.kv_heads;
+  const int batch = a.batch;
+  for (int b = 0; b < batch; b += kMaxRequests) {
+    a.batch = batch - b < kMaxRequests ? batch - b : kMaxRequests;
+    const int64_t items = pairs * a.batch;
+    e = launch_overlapped(kernel, dim3((unsigned)(items < sms ? items : sms)), dim3(C::kThreads), C::kSmem, s,
+                          dim3(1, 1), mq, mk, mv, a);
+    if (e != cudaSuccess) return e;
+    a.q_off += kMaxRequests, a.k_start += kMaxRequests, a.k_len += kMaxRequests;
+  }
+  return cudaSuccess;
+}
+
+// Prompts and documents run on the 128-row tiles, single tokens on 16-row ones.
+cudaError_t launch_attention_window(const AttnWindowArgs& a, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.max_q * (a.q_heads / a.kv_heads);
+  if (rows <= 64 || a.k_rows == 0) return launch_attention_rows(a, s);
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  if (a.head_dim == 64)
+    return a.dtype == kDtBF16 ? launch_tiles<__nv_bfloat16, 64>(a, sms, s) : launch_tiles<__half, 64>(a, sms, s);
+  return a.dtype == kDtBF16 ? launch_tiles<__nv_bfloat16, 128>(a, sms, s) : launch_tiles<__half, 128>(a, sms, s);
+}
+
+}  // namespace nemo

@@ -350,5 +350,8 @@ cudaError_t launch_forward(const FwdArgs& a, int grid, cudaStream_t s);
 // with a (box_inner x box_outer) box and 128-byte swizzle.
 int make_tmap_f16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                   uint32_t box_inner, uint32_t box_outer);
+// The same for rows row_bytes apart (a multiple of 16) of any 16-bit type.
+int make_tmap_16bit(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
+                    uint32_t box_inner, uint32_t box_outer);
 
 }  // namespace nemo
