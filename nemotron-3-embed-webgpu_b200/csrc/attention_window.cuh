@@ -62,7 +62,7 @@ struct KeyRange {
 // tile see; where such a value is infinite or NaN the product is NaN, and the
 // rows it reached are computed again here.
 template <typename T>
-__device__ __noinline__ void attention_row(const AttnWindowArgs& a, const AttnRequest& r, int i, int head, int d0,
+__device__ __noinline__ void attention_row(const AttnWindowArgs& a, AttnRequest r, int i, int head, int d0,
                                            int d1) {
   const int lane = threadIdx.x & 31, d = a.head_dim;
   const int kvh = head / (a.q_heads / a.kv_heads);

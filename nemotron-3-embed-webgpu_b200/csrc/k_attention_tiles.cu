@@ -5,46 +5,52 @@
 // two units that follow one another in the order (query tile, head of the kv
 // group), so that both read the same keys (two heads of one tile) or nearly
 // the same (neighbouring tiles), and every K and V tile it loads serves both.
-// For each unit and key tile of 128 keys:
+// For each unit and tile of 64 keys:
 //   S = Q . K^T   (tcgen05, f32 in tensor memory)
 //   online softmax by the unit's four warps, one query row per thread
 //   P = 2^(S scale log2 e - m) rounded to the 16-bit type over the columns of S
 //   O += P . V    (tcgen05, P from tensor memory, O stays there)
-// While one unit is in its softmax the tensor cores work on the other.
+// Each unit has two S tiles in tensor memory (2 x 64 columns beside 128 of O;
+// two units fill the 512): the products of the next key tile are ready when a
+// softmax ends, so neither side waits for the other's latency. (Tiles of 128
+// keys with one S took 347 us where this takes 1.)
 //
-// The window: a tile's keys start at the first visible key of the block, the
-// sinks in front of it have tiles of their own, and each product covers only
-// the 32-key chunks that some query of the unit sees. Within a tile each warp
-// leaves out the chunks that none of its 32 rows sees and masks only those
-// that some of them do not see whole.
+// The window: a block's key tiles start at its first visible key, the sinks in
+// front of it have tiles of their own, and each product covers only the 32-key
+// chunks that some query of the unit sees. Within a tile each warp leaves out
+// the chunks that none of its 32 rows sees and masks only those that some of
+// them do not see whole.
 //
-// Bound: both the tensor cores and the exponential unit need 1024 cycles per
-// 128 x 128 tile at head size 128.
+// Bound: both the tensor cores and the exponential unit need 512 cycles per
+// 128 x 64 tile at head size 128.
 //
 // Warps (320 threads, persistent, one block per SM): 0 copies Q, K and V (TMA),
 // 1 issues the products, 2-5 and 6-9 are the units' softmax. The copies and
-// first products of the next pair of units run under the last softmax and the
-// output of this one. All waits are bounded.
+// first products of the next pair of units run under the output of this one.
+// All waits are bounded.
 #include "attention_window.cuh"
 #include "kernels.cuh"
 
 namespace nemo {
 namespace {
 
-constexpr int kTile = 128;
+constexpr int kRows = 128;          // queries of a unit
+constexpr int kKeys = 64;           // keys of a tile
+constexpr int kChunks = kKeys / 32;
 constexpr int kMaxRequests = 1024;  // of one launch: their pair counts are summed in shared memory
-constexpr uint64_t kWaitNs = 20000000000ull;  // a row that is computed again key by key may hold a pair up for a while
 constexpr float kMaxSlack = 8.0f;   // the running maximum moves by more than 2^8 only: P <= 256
 
 template <int D>
 struct TilesCfg {
-  static constexpr int kHalf = kTile * 64 * 2;       // 128 rows x 64 columns, one 128-byte-swizzle block
-  static constexpr int kBlock = D / 64 * kHalf;      // 128 rows of Q, K or V
-  static constexpr int kStages = D == 64 ? 4 : 2;    // K and V tiles in flight
+  static constexpr int kQHalf = kRows * 128;     // 64 columns of Q: one 128-byte-swizzle block
+  static constexpr int kQ = D / 64 * kQHalf;
+  static constexpr int kHalf = kKeys * 128;      // 64 columns of K or V
+  static constexpr int kTileBytes = D / 64 * kHalf;
+  static constexpr int kStages = 4;              // K and V tiles in flight: two ahead of V for S, one to load
   static constexpr int kThreads = 320;
-  static constexpr int kSmem = 1024 + 2 * kBlock + kStages * 2 * kBlock + 256 + (kMaxRequests + 1) * 4;
+  static constexpr int kSmem = 1024 + 2 * kQ + kStages * 2 * kTileBytes + 256 + (kMaxRequests + 1) * 4;
   static constexpr uint32_t kTmemCols = 512;
-  static constexpr uint32_t kColS = 0, kColO = 256;  // S_t at 128 t, O_t at 256 + 128 t
+  static constexpr uint32_t kColS = 0, kColO = 256;  // S tile i of unit t at 128 t + 64 i, O_t at 256 + 128 t
 };
 
 // One unit of a block's pair.
@@ -61,14 +67,14 @@ struct Pair {
   __device__ __forceinline__ Pair(const AttnWindowArgs& a, int b, int kvh_, int pair) : rq(a, b), kvh(kvh_) {
     const int group = a.q_heads / a.kv_heads;
     const int nq = min(rq.nq, a.max_q), p_off = rq.nk - rq.nq;
-    const int units = (nq + kTile - 1) / kTile * group;
+    const int units = (nq + kRows - 1) / kRows * group;
     lo = rq.nk, hi = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int n = pair * 2 + t;
-      u[t].i0 = n / group * kTile;
+      u[t].i0 = n / group * kRows;
       u[t].head = kvh * group + n % group;
-      u[t].rows = n < units ? min(kTile, nq - u[t].i0) : 0;
+      u[t].rows = n < units ? min(kRows, nq - u[t].i0) : 0;
       u[t].lo = u[t].hi = 0;
       if (u[t].rows) {
         const KeyRange r(a, u[t].i0 + p_off, u[t].i0 + u[t].rows - 1 + p_off, rq.nk);
@@ -78,20 +84,26 @@ struct Pair {
     }
     if (lo > hi) lo = hi;
     sink = min(a.sinks, lo);
-    sink_tiles = (sink + kTile - 1) / kTile;
-    tiles = sink_tiles + (hi - lo + kTile - 1) / kTile;
+    sink_tiles = (sink + kKeys - 1) / kKeys;
+    tiles = sink_tiles + (hi - lo + kKeys - 1) / kKeys;
+  }
+  __device__ __forceinline__ Unit unit(int t) const {  // by selects: an index would put the pair into local memory
+    Unit r;
+    r.head = t ? u[1].head : u[0].head, r.i0 = t ? u[1].i0 : u[0].i0, r.rows = t ? u[1].rows : u[0].rows;
+    r.lo = t ? u[1].lo : u[0].lo, r.hi = t ? u[1].hi : u[0].hi;
+    return r;
   }
   __device__ __forceinline__ void tile(int j, int& base, int& end) const {
     if (j < sink_tiles) {
-      base = j * kTile, end = sink;
+      base = j * kKeys, end = sink;
     } else {
-      base = lo + (j - sink_tiles) * kTile, end = hi;
+      base = lo + (j - sink_tiles) * kKeys, end = hi;
     }
-    end = min(end, base + kTile);
+    end = min(end, base + kKeys);
   }
-  // The chunks [c0, c1) of 32 keys of a tile that unit t needs.
-  __device__ __forceinline__ void chunks(int t, int base, int end, int sinks, int& c0, int& c1) const {
-    const int w0 = max(base, u[t].lo), w1 = min(end, u[t].hi), s1 = min(end, min(sinks, u[t].hi));
+  // The chunks [c0, c1) of 32 keys of a tile that a unit needs.
+  __device__ __forceinline__ static void chunks(const Unit& u, int base, int end, int sinks, int& c0, int& c1) {
+    const int w0 = max(base, u.lo), w1 = min(end, u.hi), s1 = min(end, min(sinks, u.hi));
     const bool window = w1 > w0, sinked = s1 > base;
     c0 = sinked ? 0 : (w0 - base) >> 5;
     const int last = max(window ? w1 : base, sinked ? s1 : base) - base;  // keys past the last needed one
@@ -108,8 +120,10 @@ struct Items {
   __device__ __forceinline__ Pair at(const AttnWindowArgs& a, int item) {
     while (item >= before[b + 1]) ++b;  // items only grow
     const int each = (before[b + 1] - before[b]) / a.kv_heads, in = item - before[b];
-    const int kvh = in / each;
-    return Pair(a, b, kvh, each - 1 - (in - kvh * each));  // a causal request's longest pairs first
+    const int pair = in / a.kv_heads;
+    // the last queries, which see the most keys of a causal request, first: the
+    // short pairs level the blocks at the end
+    return Pair(a, b, in - pair * a.kv_heads, each - 1 - pair);
   }
   __device__ __forceinline__ int total() const { return before[batch]; }
 };
@@ -139,6 +153,31 @@ __device__ __forceinline__ uint32_t bit_range(int first, int last) {
   return from & to;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // 4 x 4 transpose of 16-byte units over each four lanes: in, unit i of the
 // lane's row; out, unit (lane & 3) of row (lane & ~3) + i.
 __device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
@@ -165,12 +204,15 @@ __global__ void __launch_bounds__(320, 1)
   const uint32_t raw_s = dev::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_s + 1023u) & ~1023u) - raw_s);
   uint8_t* sQ = smem;
-  uint8_t* sKV = sQ + 2 * C::kBlock;  // stage s: K at 2 s blocks, V behind it
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::kStages * 2 * C::kBlock);
+  uint8_t* sKV = sQ + 2 * C::kQ;  // stage s: K at 2 s tiles, V behind it
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::kStages * 2 * C::kTileBytes);
   const uint32_t q_full = dev::smem_u32(bars), q_empty = q_full + 8;
-  const uint32_t s_full = q_full + 16, p_ready = s_full + 16, pv_done = p_ready + 16, mma_fin = pv_done + 16;
+  // s_full, p_ready, pv_done: [unit][S tile]. One barrier for both S tiles would
+  // not do: a side that is a tile behind cannot tell a phase from the next but one.
+  const uint32_t s_full = q_full + 16, p_ready = s_full + 32, pv_done = p_ready + 32, mma_fin = pv_done + 32;
   const uint32_t kv_full = mma_fin + 8, kv_empty = kv_full + 8 * C::kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  uint32_t* bad = tmem_slot + 1;  // some output of this block is not finite
   int* before = reinterpret_cast<int*>(bars + 32);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -180,12 +222,13 @@ __global__ void __launch_bounds__(320, 1)
     dev::prefetch_tmap(&map_v);
     dev::mbar_init(q_full, 1);
     dev::mbar_init(q_empty, 1);
-    for (int t = 0; t < 2; ++t) {
-      dev::mbar_init(s_full + 8 * t, 1);
-      dev::mbar_init(p_ready + 8 * t, 128);
-      dev::mbar_init(pv_done + 8 * t, 1);
+    for (int i = 0; i < 4; ++i) {
+      dev::mbar_init(s_full + 8 * i, 1);
+      dev::mbar_init(p_ready + 8 * i, 128);
+      dev::mbar_init(pv_done + 8 * i, 1);
     }
     dev::mbar_init(mma_fin, 1);
+    *bad = 0;
     for (int s = 0; s < C::kStages; ++s) {
       dev::mbar_init(kv_full + 8 * s, 1);
       dev::mbar_init(kv_empty + 8 * s, 1);
@@ -209,7 +252,7 @@ __global__ void __launch_bounds__(320, 1)
       int n = 0;
       if (b < a.batch) {
         const int nq = min(AttnRequest(a, b).nq, a.max_q);
-        n = ((nq + kTile - 1) / kTile * group + 1) / 2 * a.kv_heads;
+        n = ((nq + kRows - 1) / kRows * group + 1) / 2 * a.kv_heads;
       }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -236,28 +279,29 @@ __global__ void __launch_bounds__(320, 1)
     for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
       const Pair p = items.at(a, item);
       if (!p.tiles) continue;
-      ok = __all_sync(0xffffffffu, dev::mbar_wait(q_empty, (issued_q & 1) ^ 1, a.err, kWaitNs));
+      ok = __all_sync(0xffffffffu, dev::mbar_wait(q_empty, (issued_q & 1) ^ 1, a.err));
       if (!ok) break;
       if (dev::elect_one()) {
-        dev::mbar_arrive_expect_tx(q_full, (p.u[1].rows ? 2 : 1) * C::kBlock);
+        dev::mbar_arrive_expect_tx(q_full, (p.u[1].rows ? 2 : 1) * C::kQ);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           if (p.u[t].rows)
             for (int h = 0; h < D / 64; ++h)
-              dev::tma_load_2d(dev::smem_u32(sQ + t * C::kBlock + h * C::kHalf), &map_q, p.u[t].head * D + h * 64,
+              dev::tma_load_2d(dev::smem_u32(sQ + t * C::kQ + h * C::kQHalf), &map_q, p.u[t].head * D + h * 64,
                                p.rq.q0 + p.u[t].i0, q_full);
       }
       __syncwarp();
       ++issued_q;
       for (int j = 0; j < p.tiles; ++j, ++n) {
         const int st = n % C::kStages;
-        ok = __all_sync(0xffffffffu, dev::mbar_wait(kv_empty + 8 * st, ((n / C::kStages) & 1) ^ 1, a.err, kWaitNs));
+        ok = __all_sync(0xffffffffu, dev::mbar_wait(kv_empty + 8 * st, ((n / C::kStages) & 1) ^ 1, a.err));
         if (!ok) break;
         int base, end;
         p.tile(j, base, end);
         if (dev::elect_one()) {
-          const uint32_t fb = kv_full + 8 * st, dk = dev::smem_u32(sKV + st * 2 * C::kBlock), dv = dk + C::kBlock;
-          dev::mbar_arrive_expect_tx(fb, 2 * C::kBlock);
+          const uint32_t fb = kv_full + 8 * st, dk = dev::smem_u32(sKV + st * 2 * C::kTileBytes);
+          const uint32_t dv = dk + C::kTileBytes;
+          dev::mbar_arrive_expect_tx(fb, 2 * C::kTileBytes);
           for (int h = 0; h < D / 64; ++h)
             dev::tma_load_2d(dk + h * C::kHalf, &map_k, p.kvh * D + h * 64, p.rq.k0 + base, fb);
           for (int h = 0; h < D / 64; ++h)
@@ -271,37 +315,38 @@ __global__ void __launch_bounds__(320, 1)
     for (int i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)
       dev::mbar_wait(kv_full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.err, 100000000ull);
   } else if (warp == 1) {
-    // ---- products. Per key tile j and unit t: O_t += P_t(j-1) . V(j-1)
-    // strictly before S_t(j), which overwrites P_t; the tensor pipe runs them
+    // ---- products. Step j of a pair: for each unit O += P(j) . V(j), then S
+    // of tile j + 2 into the S tile that P(j) was in; the tensor pipe runs them
     // in the order of issue ----
-    const uint32_t idesc_o = dev::make_idesc_f16(kTile, D) | idesc_type<T>() | (1u << 16);  // V MN-major
-    int n = 0, nq = 0;        // K/V tiles and Q pairs so far
-    int done[2] = {0, 0};     // softmax tiles of each unit whose P.V has been issued
+    const uint32_t idesc_o = dev::make_idesc_f16(kRows, D) | idesc_type<T>() | (1u << 16);  // V MN-major
+    int n = 0, nq = 0;    // K/V tiles before this pair, Q pairs so far
+    uint32_t s_next = 0;  // bit t: the S tile that unit t's next S goes to
+    uint32_t p_next = 0;  // bit t: the S tile that unit t's next P is in
+    uint32_t parity = 0;  // bit 2 t + i: phase of p_ready that unit t's next P.V from S tile i waits for
     bool ok = true;
     for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
       const Pair p = items.at(a, item);
       if (!p.tiles) continue;
-      ok = __all_sync(0xffffffffu, dev::mbar_wait(q_full, nq & 1, a.err, kWaitNs));
+      ok = __all_sync(0xffffffffu, dev::mbar_wait(q_full, nq & 1, a.err));
       ++nq;
-      int pend0[2], pend1[2] = {0, 0};  // chunks of the P that waits for its product with V
-      bool first[2] = {true, true};     // O_t of this pair is still empty
-      for (int j = 0; j <= p.tiles && ok; ++j) {
-        uint32_t stage = 0;
-        int base = 0, end = 0;
-        if (j < p.tiles) {
-          const int st = (n + j) % C::kStages;
-          if (!__all_sync(0xffffffffu, dev::mbar_wait(kv_full + 8 * st, ((n + j) / C::kStages) & 1, a.err, kWaitNs))) {
+      uint32_t begun = 0;  // bit t: O_t holds a product of this pair
+      for (int j = -2; j < p.tiles && ok; ++j) {
+        const int js = j + 2;  // the tile whose S is issued in this step
+        int base = 0, end = 0, base_s = 0, end_s = 0;
+        if (j >= 0) p.tile(j, base, end);
+        if (js < p.tiles) {
+          const int st = (n + js) % C::kStages;
+          if (!__all_sync(0xffffffffu, dev::mbar_wait(kv_full + 8 * st, ((n + js) / C::kStages) & 1, a.err))) {
             ok = false;
             break;
           }
-          p.tile(j, base, end);
-          stage = dev::smem_u32(sKV + st * 2 * C::kBlock);
-          const int rest = end - base;
+          p.tile(js, base_s, end_s);
+          const int rest = end_s - base_s;
           if (rest & 31) {
             // rows of V past the tile's last key, up to the end of its chunk,
             // are no request's or another one's: weight 0, but they may hold
             // infinities or NaN
-            uint8_t* v = sKV + st * 2 * C::kBlock + C::kBlock;
+            uint8_t* v = sKV + st * 2 * C::kTileBytes + C::kTileBytes;
             const int zero = ((rest + 31) & ~31) - rest;
             for (int i = lane; i < zero * 8 * (D / 64); i += 32) {
               const int h = i / (zero * 8), r = i % (zero * 8);
@@ -312,54 +357,62 @@ __global__ void __launch_bounds__(320, 1)
           }
           dev::tc_fence_after();
         }
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 2; ++t) {
-          if (!ok) break;
-          if (pend1[t]) {
-            if (!__all_sync(0xffffffffu, dev::mbar_wait(p_ready + 8 * t, done[t] & 1, a.err, kWaitNs))) {
+          const Unit u = p.unit(t);
+          int c0 = 0, c1 = 0;
+          if (j >= 0) Pair::chunks(u, base, end, a.sinks, c0, c1);
+          if (c0 < c1) {
+            const uint32_t at = 2 * t + (p_next >> t & 1);
+            if (!__all_sync(0xffffffffu, dev::mbar_wait(p_ready + 8 * at, parity >> at & 1, a.err))) {
               ok = false;
               break;
             }
-            ++done[t];
+            parity ^= 1u << at;
             dev::tc_fence_after();
-            const uint32_t v = dev::smem_u32(sKV + ((n + j - 1) % C::kStages) * 2 * C::kBlock + C::kBlock);
-            for (int kk = pend0[t] * 2; kk < pend1[t] * 2; ++kk) {
+            const uint32_t p_at = tmem + C::kColS + at * 64;
+            const uint64_t v = dev::make_sw128_desc_mn(
+                dev::smem_u32(sKV + ((n + j) % C::kStages) * 2 * C::kTileBytes + C::kTileBytes), C::kHalf, 1024);
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk) {
+              if (kk / 2 < c0 || kk / 2 >= c1) continue;
               if (dev::elect_one())
-                dev::tc_mma_f16_ts(tmem + C::kColO + t * kTile, tmem + C::kColS + t * kTile + kk * 8,
-                                   dev::make_sw128_desc_mn(v + kk * 2048, C::kHalf, 1024), idesc_o,
-                                   first[t] && kk == pend0[t] * 2 ? 0u : 1u);
+                dev::tc_mma_f16_ts(tmem + C::kColO + t * 128, p_at + kk * 8, v + kk * (2048 >> 4), idesc_o,
+                                   (begun >> t & 1) || kk > c0 * 2 ? 1u : 0u);
               __syncwarp();
             }
-            first[t] = false;
-            if (dev::elect_one()) dev::tc_commit(pv_done + 8 * t);
+            begun |= 1u << t;
+            p_next ^= 1u << t;
+            if (dev::elect_one()) dev::tc_commit(pv_done + 8 * at);
             __syncwarp();
-            pend1[t] = 0;
           }
-          if (j == p.tiles) continue;
-          int c0, c1;
-          p.chunks(t, base, end, a.sinks, c0, c1);
-          if (c0 >= c1) continue;
-          // S_t for the keys of chunks [c0, c1), at their own columns
-          const uint32_t idesc_s = dev::make_idesc_f16(kTile, (c1 - c0) * 32) | idesc_type<T>();
-          const uint32_t q = dev::smem_u32(sQ + t * C::kBlock);
+          c0 = c1 = 0;
+          if (js < p.tiles) Pair::chunks(u, base_s, end_s, a.sinks, c0, c1);
+          if (c0 < c1) {
+            // S for the keys of chunks [c0, c1), at their own columns
+            const uint32_t idesc_s = dev::make_idesc_f16(kRows, (c1 - c0) * 32) | idesc_type<T>();
+            const uint64_t qd = dev::make_sw128_desc(dev::smem_u32(sQ + t * C::kQ));
+            const uint64_t kd =
+                dev::make_sw128_desc(dev::smem_u32(sKV + ((n + js) % C::kStages) * 2 * C::kTileBytes) + c0 * 4096);
+            const uint32_t at = 2 * t + (s_next >> t & 1);
+            const uint32_t s_at = tmem + C::kColS + at * 64 + c0 * 32;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            if (dev::elect_one())
-              dev::tc_mma_f16(tmem + C::kColS + t * kTile + c0 * 32,
-                              dev::make_sw128_desc(q + (kk >> 2) * C::kHalf + (kk & 3) * 32),
-                              dev::make_sw128_desc(stage + (kk >> 2) * C::kHalf + c0 * 4096 + (kk & 3) * 32), idesc_s,
-                              kk != 0 ? 1u : 0u);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              if (dev::elect_one())
+                dev::tc_mma_f16(s_at, qd + (kk >> 2) * (C::kQHalf >> 4) + (kk & 3) * 2,
+                                kd + (kk >> 2) * (C::kHalf >> 4) + (kk & 3) * 2, idesc_s, kk != 0 ? 1u : 0u);
+              __syncwarp();
+            }
+            if (dev::elect_one()) dev::tc_commit(s_full + 8 * at);
             __syncwarp();
+            s_next ^= 1u << t;
           }
-          if (dev::elect_one()) dev::tc_commit(s_full + 8 * t);
-          __syncwarp();
-          pend0[t] = c0, pend1[t] = c1;
         }
         if (!ok) break;
-        // every product that reads tile j - 1, or the pair's Q, has been issued
-        if (j > 0 && dev::elect_one()) dev::tc_commit(kv_empty + 8 * ((n + j - 1) % C::kStages));
+        // every product that reads tile j, or the pair's Q, has been issued
+        if (j >= 0 && dev::elect_one()) dev::tc_commit(kv_empty + 8 * ((n + j) % C::kStages));
         __syncwarp();
-        if (j == p.tiles - 1 && dev::elect_one()) dev::tc_commit(q_empty);
+        if (js == p.tiles - 1 && dev::elect_one()) dev::tc_commit(q_empty);
         __syncwarp();
       }
       n += p.tiles;
@@ -371,13 +424,13 @@ __global__ void __launch_bounds__(320, 1)
     // ---- softmax of unit t: thread = query row ----
     const int t = (warp - 2) >> 2, quarter = warp & 3;
     const uint32_t rows_at = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t col_s = rows_at + C::kColS + t * kTile, col_o = rows_at + C::kColO + t * kTile;
+    const uint32_t col_o = rows_at + C::kColO + t * 128;
     const float scale = a.scale * 1.4426950408889634f;  // scores in log2 units
     int count = 0;  // tiles of this unit so far, over all pairs
     bool ok = true;
     for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
       const Pair p = items.at(a, item);
-      const Unit& u = p.u[t];
+      const Unit u = p.unit(t);
       if (!u.rows) continue;
       const int p_warp = u.i0 + quarter * 32 + p.rq.nk - p.rq.nq;
       const RowKeys mine(a, p_warp + lane, p.rq.nk), top(a, p_warp, p.rq.nk), bottom(a, p_warp + 31, p.rq.nk);
@@ -386,26 +439,28 @@ __global__ void __launch_bounds__(320, 1)
       for (int j = 0; j < p.tiles; ++j) {
         int base, end, c0, c1;
         p.tile(j, base, end);
-        p.chunks(t, base, end, a.sinks, c0, c1);
+        Pair::chunks(u, base, end, a.sinks, c0, c1);
         if (c0 >= c1) continue;
-        ok = __all_sync(0xffffffffu, dev::mbar_wait(s_full + 8 * t, count & 1, a.err, kWaitNs));
-        if (!ok) break;
-        dev::tc_fence_after();
-        float s[kTile];
         uint32_t any = 0, whole = 0;  // chunks that some row sees, that every row sees whole
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kChunks; ++c) {
           const int j0 = base + c * 32, j1 = j0 + 31;
           if (c >= c0 && c < c1 && j0 <= bottom.last && (j1 >= top.first || j0 < a.sinks)) any |= 1u << c;
           if (j1 <= top.last && j1 < end && (j0 >= bottom.first || j1 < a.sinks)) whole |= 1u << c;
         }
+        const int at = 2 * t + (count & 1);
+        const uint32_t col_s = rows_at + C::kColS + at * 64;
+        ok = __all_sync(0xffffffffu, dev::mbar_wait(s_full + 8 * at, count >> 1 & 1, a.err));
+        if (!ok) break;
+        dev::tc_fence_after();
+        float s[kKeys];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (any >> c & 1) dev::tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+        for (int c = 0; c < kChunks; ++c)
+          dev::tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
         dev::tc_wait_ld();
         float tmax = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kChunks; ++c) {
           if (!(any >> c & 1)) continue;
           if (!(whole >> c & 1)) {
             const int j0 = base + c * 32, last = min(mine.last, end - 1) - j0;
@@ -414,7 +469,7 @@ __global__ void __launch_bounds__(320, 1)
             for (int i = 0; i < 32; ++i) s[c * 32 + i] = bits >> i & 1 ? s[c * 32 + i] : -INFINITY;
           }
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) tmax = fmaxf(tmax, fmaxf(s[c * 32 + i], s[c * 32 + i + 1]));
+          for (int i = 0; i < 32; i += 2) tmax = max3(tmax, s[c * 32 + i], s[c * 32 + i + 1]);
         }
         tmax *= scale;
         // The running maximum of the warp's rows moves when some row's tile
@@ -423,19 +478,19 @@ __global__ void __launch_bounds__(320, 1)
         const bool move = __any_sync(0xffffffffu, tmax > m + kMaxSlack);
         const float mnew = move ? fmaxf(m, tmax) : m;
         const float neg = mnew == -INFINITY ? 0.f : -mnew;  // no key seen yet: all weights 0
-        const float keep = m == -INFINITY ? 0.f : dev::exp2_approx(m - mnew);
-        float sum0 = 0.f, sum1 = 0.f;
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c < c0 || c >= c1) continue;
+        for (int c = 0; c < kChunks; ++c) {
           uint32_t pr[16];
           if (any >> c & 1) {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const float e0 = dev::exp2_approx(fmaf(s[c * 32 + i], scale, neg));
-              const float e1 = dev::exp2_approx(fmaf(s[c * 32 + i + 1], scale, neg));
-              sum0 += e0, sum1 += e1;
-              pr[i / 2] = dev::pack2<T>(e0, e1);
+              float2 e = fma2(make_float2(s[c * 32 + i], s[c * 32 + i + 1]), make_float2(scale, scale),
+                              make_float2(neg, neg));
+              e.x = dev::exp2_approx(e.x);
+              e.y = dev::exp2_approx(e.y);
+              sum = add2(sum, e);
+              pr[i / 2] = dev::pack2<T>(e.x, e.y);
             }
           } else {
 #pragma unroll
@@ -443,11 +498,15 @@ __global__ void __launch_bounds__(320, 1)
           }
           tmem_st_x16(col_s + c * 16, pr);
         }
-        if (seen) {
-          // the previous tile's P.V is complete: O is stable
-          ok = __all_sync(0xffffffffu, dev::mbar_wait(pv_done + 8 * t, (count - 1) & 1, a.err, kWaitNs));
-          if (!ok) break;
-          if (move) {
+        if (move) {
+          const float keep = m == -INFINITY ? 0.f : dev::exp2_approx(m - mnew);
+          l *= keep;
+          m = mnew;
+          if (seen) {
+            // O is stable once the previous tile's P.V is complete (the one
+            // before that is: this tile's S was issued after it)
+            ok = __all_sync(0xffffffffu, dev::mbar_wait(pv_done + 8 * (at ^ 1), (count - 1) >> 1 & 1, a.err));
+            if (!ok) break;
             dev::tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
@@ -461,16 +520,16 @@ __global__ void __launch_bounds__(320, 1)
           }
         }
         dev::tc_wait_st();
-        l = l * keep + (sum0 + sum1);
-        m = mnew;
+        l += sum.x + sum.y;
         dev::tc_fence_before();
-        dev::mbar_arrive(p_ready + 8 * t);
+        dev::mbar_arrive(p_ready + 8 * at);
         ++seen;
         ++count;
       }
       if (!ok) break;
       if (seen) {
-        ok = __all_sync(0xffffffffu, dev::mbar_wait(pv_done + 8 * t, (count - 1) & 1, a.err, kWaitNs));
+        ok = __all_sync(0xffffffffu,
+                        dev::mbar_wait(pv_done + 8 * (2 * t + ((count - 1) & 1)), (count - 1) >> 1 & 1, a.err));
         if (!ok) break;
         dev::tc_fence_after();
       }
@@ -478,16 +537,13 @@ __global__ void __launch_bounds__(320, 1)
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       T* out = static_cast<T*>(a.out) + (int64_t)(p.rq.q0 + u.i0 + quarter * 32) * a.ldo + u.head * D;
       const int live = u.rows - quarter * 32;  // rows of the warp that exist
-      bool bad = false;
+      bool wrong = false;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
         if (seen) {
           dev::tmem_ld_32x32b_x32(col_o + c * 32, r);
           dev::tc_wait_ld();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0;
         }
         uint4 v[4];
 #pragma unroll
@@ -496,7 +552,7 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             y[i] = l == 0.f ? 0.f : __uint_as_float(r[k * 8 + i]) * inv;
-            bad |= !isfinite(y[i]);
+            wrong |= !isfinite(y[i]);
           }
           v[k] = dev::pack8<T>(y);
         }
@@ -507,10 +563,8 @@ __global__ void __launch_bounds__(320, 1)
           if (rr < live) *reinterpret_cast<uint4*>(out + (int64_t)rr * a.ldo + c * 32 + (lane & 3) * 8) = v[i];
         }
       }
-      if (seen) dev::tc_fence_before();  // orders the loads above before the next arrival on p_ready
-      uint32_t again = __ballot_sync(0xffffffffu, bad && lane < live);
-      for (; again; again &= again - 1)
-        attention_row<T>(a, p.rq, u.i0 + quarter * 32 + __ffs(again) - 1, u.head, 0, D);
+      dev::tc_fence_before();  // orders the loads above before the next arrival on p_ready
+      if (__any_sync(0xffffffffu, wrong && lane < live) && lane == 0) *bad = 1;
     }
   }
   dev::tc_fence_before();
@@ -518,6 +572,23 @@ __global__ void __launch_bounds__(320, 1)
   if (warp == 1) {
     dev::tc_fence_after();
     dev::tmem_dealloc(tmem, C::kTmemCols);
+  }
+  if (!*bad) return;
+  // Some row met an infinity or NaN, perhaps one that it does not see (weight 0
+  // times the value): rows whose result is not finite are computed again.
+  Items again(before, a.batch);
+  for (int item = blockIdx.x; item < total; item += gridDim.x) {
+    const Pair p = again.at(a, item);
+#pragma unroll 1
+    for (int t = 0; t < 2; ++t) {
+      const Unit u = p.unit(t);
+      for (int r = warp; r < u.rows; r += C::kThreads / 32) {
+        const T* out = static_cast<const T*>(a.out) + (int64_t)(p.rq.q0 + u.i0 + r) * a.ldo + u.head * D;
+        bool wrong = false;
+        for (int c = lane; c < D; c += 32) wrong |= !isfinite(dev::to_f32(out[c]));
+        if (__any_sync(0xffffffffu, wrong)) attention_row<T>(a, p.rq, u.i0 + r, u.head, 0, D);
+      }
+    }
   }
 }
 
@@ -538,12 +609,12 @@ static cudaError_t launch_tiles(AttnWindowArgs a, int sms, cudaStream_t s) {
     configured[dev] = true;
   }
   CUtensorMap mq, mk, mv;
-  if (make_tmap_16bit(&mq, a.q, (uint64_t)a.q_heads * D, a.q_rows, a.ldq * 2, 64, kTile) ||
-      make_tmap_16bit(&mk, a.k, (uint64_t)a.kv_heads * D, a.k_rows, a.ldk * 2, 64, kTile) ||
-      make_tmap_16bit(&mv, a.v, (uint64_t)a.kv_heads * D, a.k_rows, a.ldv * 2, 64, kTile))
+  if (make_tmap_16bit(&mq, a.q, (uint64_t)a.q_heads * D, a.q_rows, a.ldq * 2, 64, kRows) ||
+      make_tmap_16bit(&mk, a.k, (uint64_t)a.kv_heads * D, a.k_rows, a.ldk * 2, 64, kKeys) ||
+      make_tmap_16bit(&mv, a.v, (uint64_t)a.kv_heads * D, a.k_rows, a.ldv * 2, 64, kKeys))
     return cudaErrorInvalidValue;
   const int group = a.q_heads / a.kv_heads;
-  const int64_t pairs = (((int64_t)a.max_q + kTile - 1) / kTile * group + 1) / 2 * a.kv_heads;
+  const int64_t pairs = (((int64_t)a.max_q + kRows - 1) / kRows * group + 1) / 2 * a.kv_heads;
   const int batch = a.batch;
   for (int b = 0; b < batch; b += kMaxRequests) {
     a.batch = batch - b < kMaxRequests ? batch - b : kMaxRequests;
