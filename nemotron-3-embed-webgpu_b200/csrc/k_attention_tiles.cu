@@ -24,10 +24,11 @@
 // Bound: both the tensor cores and the exponential unit need 512 cycles per
 // 128 x 64 tile at head size 128.
 //
-// Warps (320 threads, persistent, one block per SM): 0 copies Q, K and V (TMA),
-// 1 issues the products, 2-5 and 6-9 are the units' softmax. The copies and
-// first products of the next pair of units run under the output of this one.
-// All waits are bounded.
+// Warps (384 threads, persistent, one block per SM): 0 copies Q, K and V (TMA),
+// 1 and 2 issue the units' products (a warp each: the tensor pipe takes one
+// unit's while the other's warp waits or finds its next tile), 4-7 and 8-11 are
+// the units' softmax. The copies and first products of the next pair of units
+// run under the output of this one. All waits are bounded.
 #include "attention_window.cuh"
 #include "kernels.cuh"
 
@@ -47,7 +48,7 @@ struct TilesCfg {
   static constexpr int kHalf = kKeys * 128;      // 64 columns of K or V
   static constexpr int kTileBytes = D / 64 * kHalf;
   static constexpr int kStages = 4;              // K and V tiles in flight: two ahead of V for S, one to load
-  static constexpr int kThreads = 320;
+  static constexpr int kThreads = 384;
   static constexpr int kSmem = 1024 + 2 * kQ + kStages * 2 * kTileBytes + 256 + (kMaxRequests + 1) * 4;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColS = 0, kColO = 256;  // S tile i of unit t at 128 t + 64 i, O_t at 256 + 128 t
@@ -196,7 +197,7 @@ __device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(384, 1)
     attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnWindowArgs a) {
   using C = TilesCfg<D>;
@@ -221,17 +222,17 @@ __global__ void __launch_bounds__(320, 1)
     dev::prefetch_tmap(&map_k);
     dev::prefetch_tmap(&map_v);
     dev::mbar_init(q_full, 1);
-    dev::mbar_init(q_empty, 1);
+    dev::mbar_init(q_empty, 2);  // both units' warps
     for (int i = 0; i < 4; ++i) {
       dev::mbar_init(s_full + 8 * i, 1);
       dev::mbar_init(p_ready + 8 * i, 128);
       dev::mbar_init(pv_done + 8 * i, 1);
     }
-    dev::mbar_init(mma_fin, 1);
+    dev::mbar_init(mma_fin, 2);
     *bad = 0;
     for (int s = 0; s < C::kStages; ++s) {
       dev::mbar_init(kv_full + 8 * s, 1);
-      dev::mbar_init(kv_empty + 8 * s, 1);
+      dev::mbar_init(kv_empty + 8 * s, 2);
     }
     dev::fence_mbar_init();
   }
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(320, 1)
     dev::tmem_alloc(dev::smem_u32(tmem_slot), C::kTmemCols);
     dev::tmem_relinquish();
   }
-  if (warp == 2) {
+  if (warp == 4) {
     // items of each request, summed by one warp
     const int group = a.q_heads / a.kv_heads;
     int sum = 0;
@@ -314,39 +315,48 @@ __global__ void __launch_bounds__(320, 1)
     if (issued_q) dev::mbar_wait(q_full, (issued_q - 1) & 1, a.err, 100000000ull);
     for (int i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)
       dev::mbar_wait(kv_full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.err, 100000000ull);
-  } else if (warp == 1) {
-    // ---- products. Step j of a pair: for each unit O += P(j) . V(j), then S
-    // of tile j + 2 into the S tile that P(j) was in; the tensor pipe runs them
-    // in the order of issue ----
-    const uint32_t idesc_o = dev::make_idesc_f16(kRows, D) | idesc_type<T>() | (1u << 16);  // V MN-major
-    int n = 0, nq = 0;    // K/V tiles before this pair, Q pairs so far
-    uint32_t s_next = 0;  // bit t: the S tile that unit t's next S goes to
-    uint32_t p_next = 0;  // bit t: the S tile that unit t's next P is in
-    uint32_t parity = 0;  // bit 2 t + i: phase of p_ready that unit t's next P.V from S tile i waits for
+  } else if (warp <= 2) {
+    // ---- products of unit t. Step js of a pair: O += P . V of tile js - 2,
+    // then S of tile js into the S tile that this P was in; the tensor pipe runs
+    // them in the order of issue. The elected lane issues each batch of products
+    // and its commit at once ----
+    const int t = warp - 1;
+    constexpr uint32_t kIdescO = dev::make_idesc_f16(kRows, D) | idesc_type<T>() | (1u << 16);  // V MN-major
+    constexpr uint32_t kIdescS = dev::make_idesc_f16(kRows, 32) | idesc_type<T>();  // one chunk; N doubles for two
+    constexpr uint32_t kN32 = 32u >> 3 << 17;
+    const uint64_t desc_q = dev::make_sw128_desc(dev::smem_u32(sQ + t * C::kQ));
+    const uint64_t desc_k = dev::make_sw128_desc(dev::smem_u32(sKV));
+    const uint64_t desc_v = dev::make_sw128_desc_mn(dev::smem_u32(sKV + C::kTileBytes), C::kHalf, 1024);
+    const uint32_t o_at = tmem + C::kColO + t * 128;
+    uint32_t n = 0, nq = 0;             // K/V tiles whose S, and Q pairs that, have been reached
+    uint32_t s_count = 0, p_count = 0;  // S tiles issued, P tiles used
     bool ok = true;
     for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
       const Pair p = items.at(a, item);
       if (!p.tiles) continue;
+      const Unit u = p.unit(t);
       ok = __all_sync(0xffffffffu, dev::mbar_wait(q_full, nq & 1, a.err));
       ++nq;
-      uint32_t begun = 0;  // bit t: O_t holds a product of this pair
-      for (int j = -2; j < p.tiles && ok; ++j) {
-        const int js = j + 2;  // the tile whose S is issued in this step
-        int base = 0, end = 0, base_s = 0, end_s = 0;
-        if (j >= 0) p.tile(j, base, end);
+      uint32_t begun = 0;  // O holds a product of this pair
+      uint32_t codes = 0;  // chunks of the tiles js - 2, js - 1, js, a byte each: c0 | c1 << 2
+      for (int js = 0; js < p.tiles + 2 && ok; ++js) {
+        const uint32_t st_s = n % C::kStages, st_v = (n - 2) % C::kStages;
+        codes >>= 8;
         if (js < p.tiles) {
-          const int st = (n + js) % C::kStages;
-          if (!__all_sync(0xffffffffu, dev::mbar_wait(kv_full + 8 * st, ((n + js) / C::kStages) & 1, a.err))) {
+          if (!__all_sync(0xffffffffu, dev::mbar_wait(kv_full + 8 * st_s, n / C::kStages & 1, a.err))) {
             ok = false;
             break;
           }
-          p.tile(js, base_s, end_s);
-          const int rest = end_s - base_s;
+          int base, end, c0, c1;
+          p.tile(js, base, end);
+          Pair::chunks(u, base, end, a.sinks, c0, c1);
+          if (c0 < c1) codes |= (uint32_t)(c0 | c1 << 2) << 16;
+          const int rest = end - base;
           if (rest & 31) {
             // rows of V past the tile's last key, up to the end of its chunk,
             // are no request's or another one's: weight 0, but they may hold
-            // infinities or NaN
-            uint8_t* v = sKV + st * 2 * C::kTileBytes + C::kTileBytes;
+            // infinities or NaN (both units' warps write the same zeros)
+            uint8_t* v = sKV + st_s * 2 * C::kTileBytes + C::kTileBytes;
             const int zero = ((rest + 31) & ~31) - rest;
             for (int i = lane; i < zero * 8 * (D / 64); i += 32) {
               const int h = i / (zero * 8), r = i % (zero * 8);
@@ -357,72 +367,63 @@ __global__ void __launch_bounds__(320, 1)
           }
           dev::tc_fence_after();
         }
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t) {
-          const Unit u = p.unit(t);
-          int c0 = 0, c1 = 0;
-          if (j >= 0) Pair::chunks(u, base, end, a.sinks, c0, c1);
-          if (c0 < c1) {
-            const uint32_t at = 2 * t + (p_next >> t & 1);
-            if (!__all_sync(0xffffffffu, dev::mbar_wait(p_ready + 8 * at, parity >> at & 1, a.err))) {
-              ok = false;
-              break;
-            }
-            parity ^= 1u << at;
-            dev::tc_fence_after();
+        const uint32_t pv = codes & 15, sc = codes >> 16;
+        if (pv) {
+          const uint32_t at = 2 * t + (p_count & 1);
+          if (!__all_sync(0xffffffffu, dev::mbar_wait(p_ready + 8 * at, p_count >> 1 & 1, a.err))) {
+            ok = false;
+            break;
+          }
+          dev::tc_fence_after();
+          if (dev::elect_one()) {
             const uint32_t p_at = tmem + C::kColS + at * 64;
-            const uint64_t v = dev::make_sw128_desc_mn(
-                dev::smem_u32(sKV + ((n + j) % C::kStages) * 2 * C::kTileBytes + C::kTileBytes), C::kHalf, 1024);
+            const uint64_t v = desc_v + st_v * (2 * C::kTileBytes >> 4);
+            uint32_t add = begun;
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk) {
-              if (kk / 2 < c0 || kk / 2 >= c1) continue;
-              if (dev::elect_one())
-                dev::tc_mma_f16_ts(tmem + C::kColO + t * 128, p_at + kk * 8, v + kk * (2048 >> 4), idesc_o,
-                                   (begun >> t & 1) || kk > c0 * 2 ? 1u : 0u);
-              __syncwarp();
+            for (int c = 0; c < kChunks; ++c) {
+              if (c < (int)(pv & 3) || c >= (int)(pv >> 2)) continue;
+              dev::tc_mma_f16_ts(o_at, p_at + c * 16, v + c * (4096 >> 4), kIdescO, add);
+              dev::tc_mma_f16_ts(o_at, p_at + c * 16 + 8, v + c * (4096 >> 4) + (2048 >> 4), kIdescO, 1);
+              add = 1;
             }
-            begun |= 1u << t;
-            p_next ^= 1u << t;
-            if (dev::elect_one()) dev::tc_commit(pv_done + 8 * at);
-            __syncwarp();
+            dev::tc_commit(pv_done + 8 * at);
           }
-          c0 = c1 = 0;
-          if (js < p.tiles) Pair::chunks(u, base_s, end_s, a.sinks, c0, c1);
-          if (c0 < c1) {
-            // S for the keys of chunks [c0, c1), at their own columns
-            const uint32_t idesc_s = dev::make_idesc_f16(kRows, (c1 - c0) * 32) | idesc_type<T>();
-            const uint64_t qd = dev::make_sw128_desc(dev::smem_u32(sQ + t * C::kQ));
-            const uint64_t kd =
-                dev::make_sw128_desc(dev::smem_u32(sKV + ((n + js) % C::kStages) * 2 * C::kTileBytes) + c0 * 4096);
-            const uint32_t at = 2 * t + (s_next >> t & 1);
-            const uint32_t s_at = tmem + C::kColS + at * 64 + c0 * 32;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              if (dev::elect_one())
-                dev::tc_mma_f16(s_at, qd + (kk >> 2) * (C::kQHalf >> 4) + (kk & 3) * 2,
-                                kd + (kk >> 2) * (C::kHalf >> 4) + (kk & 3) * 2, idesc_s, kk != 0 ? 1u : 0u);
-              __syncwarp();
-            }
-            if (dev::elect_one()) dev::tc_commit(s_full + 8 * at);
-            __syncwarp();
-            s_next ^= 1u << t;
-          }
+          __syncwarp();
+          begun = 1;
+          ++p_count;
         }
-        if (!ok) break;
-        // every product that reads tile j, or the pair's Q, has been issued
-        if (j >= 0 && dev::elect_one()) dev::tc_commit(kv_empty + 8 * ((n + j) % C::kStages));
+        if (sc) {
+          // S for the keys of the chunks, at their own columns
+          const uint32_t at = 2 * t + (s_count & 1);
+          if (dev::elect_one()) {
+            const uint32_t c0 = sc & 3, idesc = kIdescS + ((sc >> 2) - c0 - 1) * kN32;
+            const uint32_t s_at = tmem + C::kColS + at * 64 + c0 * 32;
+            const uint64_t k = desc_k + st_s * (2 * C::kTileBytes >> 4) + c0 * (4096 >> 4);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              dev::tc_mma_f16(s_at, desc_q + (kk >> 2) * (C::kQHalf >> 4) + (kk & 3) * 2,
+                              k + (kk >> 2) * (C::kHalf >> 4) + (kk & 3) * 2, idesc, kk != 0 ? 1u : 0u);
+            dev::tc_commit(s_full + 8 * at);
+          }
+          __syncwarp();
+          ++s_count;
+        }
+        // every product of the unit that reads tile js - 2, or the pair's Q, has been issued
+        if (dev::elect_one()) {
+          if (js >= 2) dev::tc_commit(kv_empty + 8 * st_v);
+          if (js == p.tiles - 1) dev::tc_commit(q_empty);
+        }
         __syncwarp();
-        if (js == p.tiles - 1 && dev::elect_one()) dev::tc_commit(q_empty);
-        __syncwarp();
+        ++n;
       }
-      n += p.tiles;
+      n -= 2;  // the last two steps had no S
     }
     if (dev::elect_one()) dev::tc_commit(mma_fin);
     __syncwarp();
     dev::mbar_wait(mma_fin, 0, a.err, 100000000ull);  // every product has retired before TMEM is freed
-  } else {
+  } else if (warp >= 4) {
     // ---- softmax of unit t: thread = query row ----
-    const int t = (warp - 2) >> 2, quarter = warp & 3;
+    const int t = (warp - 4) >> 2, quarter = warp & 3;
     const uint32_t rows_at = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t col_o = rows_at + C::kColO + t * 128;
     const float scale = a.scale * 1.4426950408889634f;  // scores in log2 units
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(320, 1)
         for (int c = 0; c < kChunks; ++c)
           dev::tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
         dev::tc_wait_ld();
-        float tmax = -INFINITY;
+        float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // maxima of independent chains
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           if (!(any >> c & 1)) continue;
@@ -469,9 +470,11 @@ __global__ void __launch_bounds__(320, 1)
             for (int i = 0; i < 32; ++i) s[c * 32 + i] = bits >> i & 1 ? s[c * 32 + i] : -INFINITY;
           }
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) tmax = max3(tmax, s[c * 32 + i], s[c * 32 + i + 1]);
+          for (int i = 0; i < 32; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) part[k] = max3(part[k], s[c * 32 + i + 2 * k], s[c * 32 + i + 2 * k + 1]);
         }
-        tmax *= scale;
+        const float tmax = scale * fmaxf(max3(part[0], part[1], part[2]), part[3]);
         // The running maximum of the warp's rows moves when some row's tile
         // maximum is more than kMaxSlack above it; otherwise P is taken
         // against the old one, at most 2^8, and O needs no rescaling.
