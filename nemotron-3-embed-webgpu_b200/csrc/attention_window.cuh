@@ -15,6 +15,7 @@ cudaError_t launch_attention_rows(const AttnWindowArgs& a, cudaStream_t s);
 struct AttnRequest {
   int q0, nq;  // first query row, queries
   int k0, nk;  // first key row, keys
+  __device__ __forceinline__ AttnRequest() {}
   __device__ __forceinline__ AttnRequest(const AttnWindowArgs& a, int b) {
     const int qa = min(max(a.q_off[b], 0), a.q_rows), qe = min(max(a.q_off[b + 1], qa), a.q_rows);
     q0 = qa;

@@ -39,6 +39,7 @@ constexpr int kRows = 128;          // queries of a unit
 constexpr int kKeys = 64;           // keys of a tile
 constexpr int kChunks = kKeys / 32;
 constexpr int kMaxRequests = 1024;  // of one launch: their pair counts are summed in shared memory
+constexpr int kListed = 48;         // items of a block that are worked out at its start
 constexpr float kMaxSlack = 8.0f;   // the running maximum moves by more than 2^8 only: P <= 256
 
 template <int D>
@@ -49,7 +50,8 @@ struct TilesCfg {
   static constexpr int kTileBytes = D / 64 * kHalf;
   static constexpr int kStages = 4;              // K and V tiles in flight: two ahead of V for S, one to load
   static constexpr int kThreads = 384;
-  static constexpr int kSmem = 1024 + 2 * kQ + kStages * 2 * kTileBytes + 256 + (kMaxRequests + 1) * 4;
+  static constexpr int kListedBytes = 96 * kListed;  // a Pair each
+  static constexpr int kSmem = 1024 + 2 * kQ + kStages * 2 * kTileBytes + 256 + kListedBytes + (kMaxRequests + 1) * 4;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColS = 0, kColO = 256;  // S tile i of unit t at 128 t + 64 i, O_t at 256 + 128 t
 };
@@ -58,13 +60,15 @@ struct TilesCfg {
 struct Unit {
   int head, i0, rows;  // q head, first query, queries (0: no such unit)
   int lo, hi;          // window keys that some query of the unit sees
+  int full0, full1;    // tiles [full0, full1) of the pair that are needed whole
 };
 
 // A pair of units and the key tiles it walks over: sink tiles first.
-struct Pair {
+struct alignas(16) Pair {
   AttnRequest rq;
   int kvh, sink, lo, hi, sink_tiles, tiles;
   Unit u[2];
+  __device__ __forceinline__ Pair() {}
   __device__ __forceinline__ Pair(const AttnWindowArgs& a, int b, int kvh_, int pair) : rq(a, b), kvh(kvh_) {
     const int group = a.q_heads / a.kv_heads;
     const int nq = min(rq.nq, a.max_q), p_off = rq.nk - rq.nq;
@@ -87,11 +91,17 @@ struct Pair {
     sink = min(a.sinks, lo);
     sink_tiles = (sink + kKeys - 1) / kKeys;
     tiles = sink_tiles + (hi - lo + kKeys - 1) / kKeys;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      u[t].full0 = sink_tiles + (max(u[t].lo - lo, 0) + kKeys - 1) / kKeys;
+      u[t].full1 = sink_tiles + max(u[t].hi - lo, 0) / kKeys;
+    }
   }
   __device__ __forceinline__ Unit unit(int t) const {  // by selects: an index would put the pair into local memory
     Unit r;
     r.head = t ? u[1].head : u[0].head, r.i0 = t ? u[1].i0 : u[0].i0, r.rows = t ? u[1].rows : u[0].rows;
     r.lo = t ? u[1].lo : u[0].lo, r.hi = t ? u[1].hi : u[0].hi;
+    r.full0 = t ? u[1].full0 : u[0].full0, r.full1 = t ? u[1].full1 : u[0].full1;
     return r;
   }
   __device__ __forceinline__ void tile(int j, int& base, int& end) const {
@@ -113,12 +123,16 @@ struct Pair {
   }
 };
 
-// Pairs of units over all requests: item -> (request, kv head, pair).
+// Pairs of units over all requests: item -> (request, kv head, pair). A block's
+// first kListed items are worked out once, in shared memory: every role reads
+// them there instead of waiting for the request's offsets between two pairs.
 struct Items {
-  const int* before;  // items of the requests before each one, [requests + 1]
+  const int* before;   // items of the requests before each one, [requests + 1]
+  const Pair* listed;  // items blockIdx.x + i * gridDim.x
   int batch, b;
-  __device__ __forceinline__ Items(const int* s, int n) : before(s), batch(n), b(0) {}
-  __device__ __forceinline__ Pair at(const AttnWindowArgs& a, int item) {
+  __device__ __forceinline__ Items(const int* s, const Pair* p, int n) : before(s), listed(p), batch(n), b(0) {}
+  __device__ __forceinline__ int total() const { return before[batch]; }
+  __device__ __forceinline__ Pair find(const AttnWindowArgs& a, int item) {
     while (item >= before[b + 1]) ++b;  // items only grow
     const int each = (before[b + 1] - before[b]) / a.kv_heads, in = item - before[b];
     const int pair = in / a.kv_heads;
@@ -126,8 +140,13 @@ struct Items {
     // short pairs level the blocks at the end
     return Pair(a, b, in - pair * a.kv_heads, each - 1 - pair);
   }
-  __device__ __forceinline__ int total() const { return before[batch]; }
+  __device__ __forceinline__ Pair at(const AttnWindowArgs& a, int item) {
+    const int i = (item - blockIdx.x) / gridDim.x;
+    return i < kListed ? listed[i] : find(a, item);
+  }
 };
+
+static_assert(sizeof(Pair) == 96, "kListedBytes");
 
 template <typename T>
 constexpr uint32_t idesc_type() {
@@ -179,21 +198,18 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-// 4 x 4 transpose of 16-byte units over each four lanes: in, unit i of the
-// lane's row; out, unit (lane & 3) of row (lane & ~3) + i.
-__device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
-  auto swap = [&](uint4& x, uint4& y, int mask, bool up) {  // the lane with the bit set gives x, the other one y
-    uint4 s = up ? x : y;
-    s.x = __shfl_xor_sync(0xffffffffu, s.x, mask);
-    s.y = __shfl_xor_sync(0xffffffffu, s.y, mask);
-    s.z = __shfl_xor_sync(0xffffffffu, s.z, mask);
-    s.w = __shfl_xor_sync(0xffffffffu, s.w, mask);
-    (up ? x : y) = s;
-  };
-  swap(v[0], v[1], 1, lane & 1);
-  swap(v[2], v[3], 1, lane & 1);
-  swap(v[0], v[2], 2, lane & 2);
-  swap(v[1], v[3], 2, lane & 2);
+// One 32-byte store: a whole sector of a thread's own row. Rows are 16-byte
+// aligned only; those that are not 32-byte aligned take two stores.
+template <typename T>
+__device__ __forceinline__ void store32(T* p, const uint32_t* v) {
+  if (((uintptr_t)p & 31) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
 }
 
 template <typename T, int D>
@@ -211,10 +227,11 @@ __global__ void __launch_bounds__(384, 1)
   // s_full, p_ready, pv_done: [unit][S tile]. One barrier for both S tiles would
   // not do: a side that is a tile behind cannot tell a phase from the next but one.
   const uint32_t s_full = q_full + 16, p_ready = s_full + 32, pv_done = p_ready + 32, mma_fin = pv_done + 32;
-  const uint32_t kv_full = mma_fin + 8, kv_empty = kv_full + 8 * C::kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  const uint32_t kv_full = mma_fin + 8, kv_ready = kv_full + 8 * C::kStages, kv_empty = kv_ready + 8 * C::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
   uint32_t* bad = tmem_slot + 1;  // some output of this block is not finite
-  int* before = reinterpret_cast<int*>(bars + 32);
+  Pair* listed = reinterpret_cast<Pair*>(bars + 32);
+  int* before = reinterpret_cast<int*>(bars + 32) + C::kListedBytes / 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 0 && lane == 0) {
@@ -232,6 +249,7 @@ __global__ void __launch_bounds__(384, 1)
     *bad = 0;
     for (int s = 0; s < C::kStages; ++s) {
       dev::mbar_init(kv_full + 8 * s, 1);
+      dev::mbar_init(kv_ready + 8 * s, 1);
       dev::mbar_init(kv_empty + 8 * s, 2);
     }
     dev::fence_mbar_init();
@@ -270,8 +288,14 @@ __global__ void __launch_bounds__(384, 1)
   dev::tc_fence_after();
   dev::pdl_launch_dependents();
   const uint32_t tmem = *tmem_slot;
-  Items items(before, a.batch);
+  Items items(before, listed, a.batch);
   const int total = items.total();
+  if (threadIdx.x < kListed) {
+    Items mine(before, listed, a.batch);
+    const int item = blockIdx.x + threadIdx.x * gridDim.x;
+    if (item < total) listed[threadIdx.x] = mine.find(a, item);
+  }
+  __syncthreads();
 
   if (warp == 0) {
     // ---- copies: the elected lane of the converged warp issues them ----
@@ -316,86 +340,66 @@ __global__ void __launch_bounds__(384, 1)
     for (int i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)
       dev::mbar_wait(kv_full + 8 * (i % C::kStages), (i / C::kStages) & 1, a.err, 100000000ull);
   } else if (warp <= 2) {
-    // ---- products of unit t. Step js of a pair: O += P . V of tile js - 2,
-    // then S of tile js into the S tile that this P was in; the tensor pipe runs
-    // them in the order of issue. The elected lane issues each batch of products
-    // and its commit at once ----
-    const int t = warp - 1;
-    constexpr uint32_t kIdescO = dev::make_idesc_f16(kRows, D) | idesc_type<T>() | (1u << 16);  // V MN-major
-    constexpr uint32_t kIdescS = dev::make_idesc_f16(kRows, 32) | idesc_type<T>();  // one chunk; N doubles for two
-    constexpr uint32_t kN32 = 32u >> 3 << 17;
-    const uint64_t desc_q = dev::make_sw128_desc(dev::smem_u32(sQ + t * C::kQ));
-    const uint64_t desc_k = dev::make_sw128_desc(dev::smem_u32(sKV));
-    const uint64_t desc_v = dev::make_sw128_desc_mn(dev::smem_u32(sKV + C::kTileBytes), C::kHalf, 1024);
-    const uint32_t o_at = tmem + C::kColO + t * 128;
-    uint32_t n = 0, nq = 0;             // K/V tiles whose S, and Q pairs that, have been reached
-    uint32_t s_count = 0, p_count = 0;  // S tiles issued, P tiles used
-    bool ok = true;
-    for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
-      const Pair p = items.at(a, item);
-      if (!p.tiles) continue;
-      const Unit u = p.unit(t);
-      ok = __all_sync(0xffffffffu, dev::mbar_wait(q_full, nq & 1, a.err));
-      ++nq;
-      uint32_t begun = 0;  // O holds a product of this pair
-      uint32_t codes = 0;  // chunks of the tiles js - 2, js - 1, js, a byte each: c0 | c1 << 2
-      for (int js = 0; js < p.tiles + 2 && ok; ++js) {
-        const uint32_t st_s = n % C::kStages, st_v = (n - 2) % C::kStages;
-        codes >>= 8;
-        if (js < p.tiles) {
-          if (!__all_sync(0xffffffffu, dev::mbar_wait(kv_full + 8 * st_s, n / C::kStages & 1, a.err))) {
-            ok = false;
-            break;
-          }
-          int base, end, c0, c1;
-          p.tile(js, base, end);
-          Pair::chunks(u, base, end, a.sinks, c0, c1);
-          if (c0 < c1) codes |= (uint32_t)(c0 | c1 << 2) << 16;
-          const int rest = end - base;
-          if (rest & 31) {
-            // rows of V past the tile's last key, up to the end of its chunk,
-            // are no request's or another one's: weight 0, but they may hold
-            // infinities or NaN (both units' warps write the same zeros)
-            uint8_t* v = sKV + st_s * 2 * C::kTileBytes + C::kTileBytes;
-            const int zero = ((rest + 31) & ~31) - rest;
-            for (int i = lane; i < zero * 8 * (D / 64); i += 32) {
-              const int h = i / (zero * 8), r = i % (zero * 8);
-              *reinterpret_cast<uint4*>(v + h * C::kHalf + rest * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+    // ---- products of unit t, by one thread. Step js of a pair: O += P . V of
+    // tile js - 2, then S of tile js into the S tile that this P was in; the
+    // tensor pipe runs them in the order of issue ----
+    if (dev::elect_one()) {
+      const int t = warp - 1;
+      constexpr uint32_t kIdescO = dev::make_idesc_f16(kRows, D) | idesc_type<T>() | (1u << 16);  // V MN-major
+      constexpr uint32_t kIdescS = dev::make_idesc_f16(kRows, 32) | idesc_type<T>();  // one chunk; N doubles for two
+      constexpr uint32_t kN32 = 32u >> 3 << 17;
+      const uint64_t desc_q = dev::make_sw128_desc(dev::smem_u32(sQ + t * C::kQ));
+      const uint64_t desc_k = dev::make_sw128_desc(dev::smem_u32(sKV));
+      const uint64_t desc_v = dev::make_sw128_desc_mn(dev::smem_u32(sKV + C::kTileBytes), C::kHalf, 1024);
+      const uint32_t o_at = tmem + C::kColO + t * 128;
+      constexpr uint32_t kWhole = kChunks << 2;  // the code of a tile that is needed whole
+      uint32_t n = 0, nq = 0;                    // K/V tiles whose S, and Q pairs that, have been reached
+      uint32_t s_count = 0, p_count = 0;         // S tiles issued, P tiles used
+      bool ok = true;
+      for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
+        const Pair p = items.at(a, item);
+        if (!p.tiles) continue;
+        const Unit u = p.unit(t);
+        if (!dev::mbar_wait(q_full, nq & 1, a.err)) break;
+        ++nq;
+        uint32_t begun = 0;  // O holds a product of this pair
+        uint32_t codes = 0;  // chunks of the tiles js - 2, js - 1, js, a byte each: c0 | c1 << 2
+        for (int js = 0; js < p.tiles + 2; ++js, ++n) {
+          const uint32_t st_s = n % C::kStages, st_v = (n - 2) % C::kStages;
+          codes >>= 8;
+          if (js < p.tiles) {
+            if (js >= u.full0 && js < u.full1) {
+              codes |= kWhole << 16;
+            } else {
+              int base, end, c0, c1;
+              p.tile(js, base, end);
+              Pair::chunks(u, base, end, a.sinks, c0, c1);
+              if (c0 < c1) codes |= (uint32_t)(c0 | c1 << 2) << 16;
             }
-            dev::fence_proxy_async_smem();
-            __syncwarp();
+            ok = dev::mbar_wait(kv_ready + 8 * st_s, n / C::kStages & 1, a.err);
+            if (!ok) break;
           }
-          dev::tc_fence_after();
-        }
-        const uint32_t pv = codes & 15, sc = codes >> 16;
-        if (pv) {
-          const uint32_t at = 2 * t + (p_count & 1);
-          if (!__all_sync(0xffffffffu, dev::mbar_wait(p_ready + 8 * at, p_count >> 1 & 1, a.err))) {
-            ok = false;
-            break;
-          }
-          dev::tc_fence_after();
-          if (dev::elect_one()) {
+          const uint32_t pv = codes & 15, sc = codes >> 16;
+          if (pv) {
+            const uint32_t at = 2 * t + (p_count & 1);
+            ok = dev::mbar_wait(p_ready + 8 * at, p_count >> 1 & 1, a.err);
+            if (!ok) break;
+            dev::tc_fence_after();
             const uint32_t p_at = tmem + C::kColS + at * 64;
             const uint64_t v = desc_v + st_v * (2 * C::kTileBytes >> 4);
-            uint32_t add = begun;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
-              if (c < (int)(pv & 3) || c >= (int)(pv >> 2)) continue;
-              dev::tc_mma_f16_ts(o_at, p_at + c * 16, v + c * (4096 >> 4), kIdescO, add);
+              if (pv != kWhole && (c < (int)(pv & 3) || c >= (int)(pv >> 2))) continue;
+              dev::tc_mma_f16_ts(o_at, p_at + c * 16, v + c * (4096 >> 4), kIdescO, begun);
               dev::tc_mma_f16_ts(o_at, p_at + c * 16 + 8, v + c * (4096 >> 4) + (2048 >> 4), kIdescO, 1);
-              add = 1;
+              begun = 1;
             }
             dev::tc_commit(pv_done + 8 * at);
+            ++p_count;
           }
-          __syncwarp();
-          begun = 1;
-          ++p_count;
-        }
-        if (sc) {
-          // S for the keys of the chunks, at their own columns
-          const uint32_t at = 2 * t + (s_count & 1);
-          if (dev::elect_one()) {
+          if (sc) {
+            // S for the keys of the chunks, at their own columns
+            const uint32_t at = 2 * t + (s_count & 1);
             const uint32_t c0 = sc & 3, idesc = kIdescS + ((sc >> 2) - c0 - 1) * kN32;
             const uint32_t s_at = tmem + C::kColS + at * 64 + c0 * 32;
             const uint64_t k = desc_k + st_s * (2 * C::kTileBytes >> 4) + c0 * (4096 >> 4);
@@ -404,24 +408,48 @@ __global__ void __launch_bounds__(384, 1)
               dev::tc_mma_f16(s_at, desc_q + (kk >> 2) * (C::kQHalf >> 4) + (kk & 3) * 2,
                               k + (kk >> 2) * (C::kHalf >> 4) + (kk & 3) * 2, idesc, kk != 0 ? 1u : 0u);
             dev::tc_commit(s_full + 8 * at);
+            ++s_count;
           }
-          __syncwarp();
-          ++s_count;
-        }
-        // every product of the unit that reads tile js - 2, or the pair's Q, has been issued
-        if (dev::elect_one()) {
+          // every product of the unit that reads tile js - 2, or the pair's Q, has been issued
           if (js >= 2) dev::tc_commit(kv_empty + 8 * st_v);
           if (js == p.tiles - 1) dev::tc_commit(q_empty);
         }
-        __syncwarp();
-        ++n;
+        n -= 2;  // the last two steps had no S
       }
-      n -= 2;  // the last two steps had no S
+      dev::tc_commit(mma_fin);
     }
-    if (dev::elect_one()) dev::tc_commit(mma_fin);
     __syncwarp();
     dev::mbar_wait(mma_fin, 0, a.err, 100000000ull);  // every product has retired before TMEM is freed
-  } else if (warp >= 4) {
+  } else if (warp == 3) {
+    // ---- passes each K/V tile on to the products. Rows of V past a tile's last
+    // key, up to the end of its 32-key chunk, are no request's or another one's:
+    // their weights are 0, but they may hold infinities or NaN, so they become
+    // zeros first ----
+    uint32_t n = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
+      const Pair p = items.at(a, item);
+      for (int j = 0; j < p.tiles; ++j, ++n) {
+        const uint32_t st = n % C::kStages;
+        ok = __all_sync(0xffffffffu, dev::mbar_wait(kv_full + 8 * st, n / C::kStages & 1, a.err));
+        if (!ok) break;
+        int base, end;
+        p.tile(j, base, end);
+        const int keys = end - base;
+        if (keys & 31) {
+          uint8_t* v = sKV + st * 2 * C::kTileBytes + C::kTileBytes;
+          const int zero = ((keys + 31) & ~31) - keys;
+          for (int i = lane; i < zero * 8 * (D / 64); i += 32) {
+            const int h = i / (zero * 8), r = i % (zero * 8);
+            *reinterpret_cast<uint4*>(v + h * C::kHalf + keys * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+          }
+          dev::fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) dev::mbar_arrive(kv_ready + 8 * st);
+      }
+    }
+  } else {
     // ---- softmax of unit t: thread = query row ----
     const int t = (warp - 4) >> 2, quarter = warp & 3;
     const uint32_t rows_at = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -435,19 +463,26 @@ __global__ void __launch_bounds__(384, 1)
       if (!u.rows) continue;
       const int p_warp = u.i0 + quarter * 32 + p.rq.nk - p.rq.nq;
       const RowKeys mine(a, p_warp + lane, p.rq.nk), top(a, p_warp, p.rq.nk), bottom(a, p_warp + 31, p.rq.nk);
+      // Window tiles [plain0, plain1) whose 64 keys every row of the warp sees.
+      const int plain0 = p.sink_tiles + (max(bottom.first - p.lo, 0) + kKeys - 1) / kKeys;
+      const int plain1 = p.sink_tiles + max(min(top.last + 1, u.hi) - p.lo, 0) / kKeys;
       float m = -INFINITY, l = 0.f;
       int seen = 0;  // tiles of this pair
       for (int j = 0; j < p.tiles; ++j) {
-        int base, end, c0, c1;
-        p.tile(j, base, end);
-        Pair::chunks(u, base, end, a.sinks, c0, c1);
-        if (c0 >= c1) continue;
-        uint32_t any = 0, whole = 0;  // chunks that some row sees, that every row sees whole
+        int base = 0, end = 0;
+        uint32_t any = 3, whole = 3;  // chunks that some row sees, that every row sees whole
+        if (j < plain0 || j >= plain1) {
+          int c0, c1;
+          p.tile(j, base, end);
+          Pair::chunks(u, base, end, a.sinks, c0, c1);
+          if (c0 >= c1) continue;
+          any = whole = 0;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int j0 = base + c * 32, j1 = j0 + 31;
-          if (c >= c0 && c < c1 && j0 <= bottom.last && (j1 >= top.first || j0 < a.sinks)) any |= 1u << c;
-          if (j1 <= top.last && j1 < end && (j0 >= bottom.first || j1 < a.sinks)) whole |= 1u << c;
+          for (int c = 0; c < kChunks; ++c) {
+            const int j0 = base + c * 32, j1 = j0 + 31;
+            if (c >= c0 && c < c1 && j0 <= bottom.last && (j1 >= top.first || j0 < a.sinks)) any |= 1u << c;
+            if (j1 <= top.last && j1 < end && (j0 >= bottom.first || j1 < a.sinks)) whole |= 1u << c;
+          }
         }
         const int at = 2 * t + (count & 1);
         const uint32_t col_s = rows_at + C::kColS + at * 64;
@@ -455,73 +490,88 @@ __global__ void __launch_bounds__(384, 1)
         if (!ok) break;
         dev::tc_fence_after();
         float s[kKeys];
+        uint32_t pr[kKeys / 2];
+        float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // maxima of independent chains
+        float2 sum = make_float2(0.f, 0.f);
+        bool done = false;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
           dev::tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
         dev::tc_wait_ld();
-        float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // maxima of independent chains
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          if (!(any >> c & 1)) continue;
-          if (!(whole >> c & 1)) {
-            const int j0 = base + c * 32, last = min(mine.last, end - 1) - j0;
-            const uint32_t bits = bit_range(mine.first - j0, last) | bit_range(0, min(last, a.sinks - 1 - j0));
-#pragma unroll
-            for (int i = 0; i < 32; ++i) s[c * 32 + i] = bits >> i & 1 ? s[c * 32 + i] : -INFINITY;
-          }
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) part[k] = max3(part[k], s[c * 32 + i + 2 * k], s[c * 32 + i + 2 * k + 1]);
-        }
-        const float tmax = scale * fmaxf(max3(part[0], part[1], part[2]), part[3]);
         // The running maximum of the warp's rows moves when some row's tile
-        // maximum is more than kMaxSlack above it; otherwise P is taken
-        // against the old one, at most 2^8, and O needs no rescaling.
-        const bool move = __any_sync(0xffffffffu, tmax > m + kMaxSlack);
-        const float mnew = move ? fmaxf(m, tmax) : m;
-        const float neg = mnew == -INFINITY ? 0.f : -mnew;  // no key seen yet: all weights 0
-        float2 sum = make_float2(0.f, 0.f);
+        // maximum is more than kMaxSlack above it; otherwise P is taken against
+        // the old one, at most 2^8, and O needs no rescaling. A tile that every
+        // row sees takes its weights against the old maximum straight away, with
+        // its own maximum found beside them, and again only where it moves.
+        if (any == 3 && whole == 3 && seen) {
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          uint32_t pr[16];
-          if (any >> c & 1) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float2 e = fma2(make_float2(s[c * 32 + i], s[c * 32 + i + 1]), make_float2(scale, scale),
-                              make_float2(neg, neg));
-              e.x = dev::exp2_approx(e.x);
-              e.y = dev::exp2_approx(e.y);
-              sum = add2(sum, e);
-              pr[i / 2] = dev::pack2<T>(e.x, e.y);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pr[i] = 0;
+          for (int i = 0; i < kKeys; i += 2) {
+            part[i / 2 % 4] = max3(part[i / 2 % 4], s[i], s[i + 1]);
+            const float2 x = fma2(make_float2(s[i], s[i + 1]), make_float2(scale, scale), make_float2(-m, -m));
+            const float2 e = make_float2(dev::exp2_approx(x.x), dev::exp2_approx(x.y));
+            sum = add2(sum, e);
+            pr[i / 2] = dev::pack2<T>(e.x, e.y);
           }
-          tmem_st_x16(col_s + c * 16, pr);
+          const float tmax = scale * fmaxf(max3(part[0], part[1], part[2]), part[3]);
+          done = !__any_sync(0xffffffffu, tmax > m + kMaxSlack || m == -INFINITY);
         }
-        if (move) {
-          const float keep = m == -INFINITY ? 0.f : dev::exp2_approx(m - mnew);
-          l *= keep;
-          m = mnew;
-          if (seen) {
-            // O is stable once the previous tile's P.V is complete (the one
-            // before that is: this tile's S was issued after it)
-            ok = __all_sync(0xffffffffu, dev::mbar_wait(pv_done + 8 * (at ^ 1), (count - 1) >> 1 & 1, a.err));
-            if (!ok) break;
-            dev::tc_fence_after();
+        if (!done) {
+          sum = make_float2(0.f, 0.f);
+          float tmax = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              dev::tmem_ld_32x32b_x32(col_o + c * 32, o);
-              dev::tc_wait_ld();
+          for (int c = 0; c < kChunks; ++c) {
+            if (!(any >> c & 1)) continue;
+            if (!(whole >> c & 1)) {
+              const int j0 = base + c * 32, last = min(mine.last, end - 1) - j0;
+              const uint32_t bits = bit_range(mine.first - j0, last) | bit_range(0, min(last, a.sinks - 1 - j0));
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-              dev::tmem_st_32x32b_x32(col_o + c * 32, o);
+              for (int i = 0; i < 32; ++i) s[c * 32 + i] = bits >> i & 1 ? s[c * 32 + i] : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) tmax = max3(tmax, s[c * 32 + i], s[c * 32 + i + 1]);
+          }
+          tmax *= scale;
+          const bool move = __any_sync(0xffffffffu, tmax > m + kMaxSlack);
+          const float mnew = move ? fmaxf(m, tmax) : m;
+          const float neg = mnew == -INFINITY ? 0.f : -mnew;  // no key seen yet: all weights 0
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            if (any >> c & 1) {
+#pragma unroll
+              for (int i = c * 32; i < c * 32 + 32; i += 2) {
+                const float2 x = fma2(make_float2(s[i], s[i + 1]), make_float2(scale, scale), make_float2(neg, neg));
+                const float2 e = make_float2(dev::exp2_approx(x.x), dev::exp2_approx(x.y));
+                sum = add2(sum, e);
+                pr[i / 2] = dev::pack2<T>(e.x, e.y);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pr[c * 16 + i] = 0;
+            }
+          }
+          if (move) {
+            const float keep = m == -INFINITY ? 0.f : dev::exp2_approx(m - mnew);
+            l *= keep;
+            m = mnew;
+            if (seen) {
+              // O is stable once the previous tile's P.V is complete (the one
+              // before that is: this tile's S was issued after it)
+              ok = __all_sync(0xffffffffu, dev::mbar_wait(pv_done + 8 * (at ^ 1), (count - 1) >> 1 & 1, a.err));
+              if (!ok) break;
+              dev::tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                dev::tmem_ld_32x32b_x16(col_o + c * 16, o);
+                dev::tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                tmem_st_x16(col_o + c * 16, o);
+              }
             }
           }
         }
+        dev::tmem_st_32x32b_x32(col_s, pr);
         dev::tc_wait_st();
         l += sum.x + sum.y;
         dev::tc_fence_before();
@@ -536,38 +586,37 @@ __global__ void __launch_bounds__(384, 1)
         if (!ok) break;
         dev::tc_fence_after();
       }
-      // output: O / l, four lanes writing 64 bytes of a row at a time
+      // output: O / l, one row per thread in 32-byte stores
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      T* out = static_cast<T*>(a.out) + (int64_t)(p.rq.q0 + u.i0 + quarter * 32) * a.ldo + u.head * D;
-      const int live = u.rows - quarter * 32;  // rows of the warp that exist
-      bool wrong = false;
+      const int row = u.i0 + quarter * 32 + lane;
+      const bool live = quarter * 32 + lane < u.rows;
+      T* out = static_cast<T*>(a.out) + (int64_t)(p.rq.q0 + row) * a.ldo + u.head * D;
+      float2 probe = make_float2(0.f, 0.f);  // stays 0 unless some value is infinite or NaN
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
+        float o[32];
         if (seen) {
-          dev::tmem_ld_32x32b_x32(col_o + c * 32, r);
+          dev::tmem_ld_32x32b_x32(col_o + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
           dev::tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
         }
-        uint4 v[4];
+        uint32_t v[16];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float y[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            y[i] = l == 0.f ? 0.f : __uint_as_float(r[k * 8 + i]) * inv;
-            wrong |= !isfinite(y[i]);
-          }
-          v[k] = dev::pack8<T>(y);
+        for (int i = 0; i < 16; ++i) {
+          // a row that has seen nothing has zeros there (0 times finite values) or garbage times inv = 0
+          const float2 y = fma2(make_float2(o[2 * i], o[2 * i + 1]), make_float2(inv, inv), make_float2(0.f, 0.f));
+          probe = fma2(y, make_float2(0.f, 0.f), probe);
+          v[i] = dev::pack2<T>(y.x, y.y);
         }
-        transpose4(v, lane);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int rr = (lane & ~3) + i;
-          if (rr < live) *reinterpret_cast<uint4*>(out + (int64_t)rr * a.ldo + c * 32 + (lane & 3) * 8) = v[i];
+        if (live) {
+          store32(out + c * 32, v);
+          store32(out + c * 32 + 16, v + 8);
         }
       }
       dev::tc_fence_before();  // orders the loads above before the next arrival on p_ready
-      if (__any_sync(0xffffffffu, wrong && lane < live) && lane == 0) *bad = 1;
+      if (__any_sync(0xffffffffu, live && !(probe.x + probe.y == 0.f)) && lane == 0) *bad = 1;
     }
   }
   dev::tc_fence_before();
@@ -579,7 +628,7 @@ __global__ void __launch_bounds__(384, 1)
   if (!*bad) return;
   // Some row met an infinity or NaN, perhaps one that it does not see (weight 0
   // times the value): rows whose result is not finite are computed again.
-  Items again(before, a.batch);
+  Items again(before, listed, a.batch);
   for (int item = blockIdx.x; item < total; item += gridDim.x) {
     const Pair p = again.at(a, item);
 #pragma unroll 1

@@ -272,6 +272,29 @@ def test_attention_window_garbage_in_unseen_keys(gen, dt, q_len):
     ref.close(got[fine], ref_got[fine].double(), 4 * ref.HALF[dt] * clean[1].abs().max().double())
 
 
+@TYPES
+@pytest.mark.parametrize("q_len", [3, 260])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_attention_window_bad_keys_in_the_open(gen, dt, q_len, bad):
+    """One key that every query sees, at each place of a 64-key tile in turn (one kv head each): NaN and infinite
+    scores make every row of that head NaN or, for a score of -inf, count for nothing; the clean head stays clean."""
+    hk, nk = 65, 700
+    args = packed(gen, dt, [q_len], [nk], hk, hk, 64)
+    q, k, v = args[:3]
+    q.abs_()
+    for h in range(64):
+        k[128 + h, h] = bad
+    got = ref.attention(*args, -1, -1, 0)
+    if bad == -float("inf"):
+        assert torch.isfinite(got).all()
+        k[:, :64] = torch.where(torch.isinf(k[:, :64]), -1000.0, k[:, :64])  # no weight either
+        ref.check_attention(*args, -1, -1, 0, got)
+    else:
+        assert not torch.isfinite(got[:, :64]).any()
+        one = (q[:, 64:].contiguous(), k[:, 64:].contiguous(), v[:, 64:].contiguous(), *args[3:])
+        ref.check_attention(*one, -1, -1, 0, got[:, 64:])
+
+
 @pytest.mark.parametrize("q_len", [1, 200])
 def test_attention_window_large_scores(gen, q_len):
     """Scores of several thousand: the largest key takes all the weight, nothing overflows."""
