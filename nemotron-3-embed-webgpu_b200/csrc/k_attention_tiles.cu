@@ -40,7 +40,8 @@ constexpr int kKeys = 64;           // keys of a tile
 constexpr int kChunks = kKeys / 32;
 constexpr int kMaxRequests = 1024;  // of one launch: their pair counts are summed in shared memory
 constexpr int kListed = 48;         // items of a block that are worked out at its start
-constexpr float kMaxSlack = 8.0f;   // the running maximum moves by more than 2^8 only: P <= 256
+constexpr float kMaxSum = 256.0f;   // sum of a row's weights of one tile against an old maximum, at most
+constexpr float kMaxSlack = 8.0f;   // and how far such a maximum may be exceeded (log2)
 
 template <int D>
 struct TilesCfg {
@@ -491,29 +492,28 @@ __global__ void __launch_bounds__(384, 1)
         dev::tc_fence_after();
         float s[kKeys];
         uint32_t pr[kKeys / 2];
-        float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // maxima of independent chains
-        float2 sum = make_float2(0.f, 0.f);
+        float2 sum = make_float2(0.f, 0.f), sum1 = sum;
         bool done = false;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
           dev::tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
         dev::tc_wait_ld();
-        // The running maximum of the warp's rows moves when some row's tile
-        // maximum is more than kMaxSlack above it; otherwise P is taken against
-        // the old one, at most 2^8, and O needs no rescaling. A tile that every
-        // row sees takes its weights against the old maximum straight away, with
-        // its own maximum found beside them, and again only where it moves.
+        // A tile that every row sees takes its weights against the running maximum
+        // straight away. They stand if every row's sum is at most 2^8: then no
+        // weight is above that either, far inside the 16-bit types, and O needs no
+        // rescaling. Otherwise the tile's own maximum is found, the running one
+        // moves and the weights are taken again. (A NaN fails the comparison.)
         if (any == 3 && whole == 3 && seen) {
 #pragma unroll
           for (int i = 0; i < kKeys; i += 2) {
-            part[i / 2 % 4] = max3(part[i / 2 % 4], s[i], s[i + 1]);
             const float2 x = fma2(make_float2(s[i], s[i + 1]), make_float2(scale, scale), make_float2(-m, -m));
             const float2 e = make_float2(dev::exp2_approx(x.x), dev::exp2_approx(x.y));
-            sum = add2(sum, e);
+            if (i & 2) sum1 = add2(sum1, e);
+            else sum = add2(sum, e);
             pr[i / 2] = dev::pack2<T>(e.x, e.y);
           }
-          const float tmax = scale * fmaxf(max3(part[0], part[1], part[2]), part[3]);
-          done = !__any_sync(0xffffffffu, tmax > m + kMaxSlack || m == -INFINITY);
+          sum = add2(sum, sum1);
+          done = __all_sync(0xffffffffu, sum.x + sum.y <= kMaxSum);
         }
         if (!done) {
           sum = make_float2(0.f, 0.f);
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(384, 1)
             for (int i = 0; i < 32; i += 2) tmax = max3(tmax, s[c * 32 + i], s[c * 32 + i + 1]);
           }
           tmax *= scale;
-          const bool move = __any_sync(0xffffffffu, tmax > m + kMaxSlack);
+          const bool move = __any_sync(0xffffffffu, tmax > m + (whole == 3 ? 0.f : kMaxSlack));
           const float mnew = move ? fmaxf(m, tmax) : m;
           const float neg = mnew == -INFINITY ? 0.f : -mnew;  // no key seen yet: all weights 0
 #pragma unroll
