@@ -174,31 +174,6 @@ __device__ __forceinline__ uint32_t bit_range(int first, int last) {
   return from & to;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// Two f32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
-      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, w;\n\t"
-      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 // One 32-byte store: a whole sector of a thread's own row. Rows are 16-byte
 // aligned only; those that are not 32-byte aligned take two stores.
 template <typename T>
@@ -506,13 +481,13 @@ __global__ void __launch_bounds__(384, 1)
         if (any == 3 && whole == 3 && seen) {
 #pragma unroll
           for (int i = 0; i < kKeys; i += 2) {
-            const float2 x = fma2(make_float2(s[i], s[i + 1]), make_float2(scale, scale), make_float2(-m, -m));
+            const float2 x = dev::fma2(make_float2(s[i], s[i + 1]), make_float2(scale, scale), make_float2(-m, -m));
             const float2 e = make_float2(dev::exp2_approx(x.x), dev::exp2_approx(x.y));
-            if (i & 2) sum1 = add2(sum1, e);
-            else sum = add2(sum, e);
+            if (i & 2) sum1 = dev::add2(sum1, e);
+            else sum = dev::add2(sum, e);
             pr[i / 2] = dev::pack2<T>(e.x, e.y);
           }
-          sum = add2(sum, sum1);
+          sum = dev::add2(sum, sum1);
           done = __all_sync(0xffffffffu, sum.x + sum.y <= kMaxSum);
         }
         if (!done) {
@@ -528,7 +503,7 @@ __global__ void __launch_bounds__(384, 1)
               for (int i = 0; i < 32; ++i) s[c * 32 + i] = bits >> i & 1 ? s[c * 32 + i] : -INFINITY;
             }
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) tmax = max3(tmax, s[c * 32 + i], s[c * 32 + i + 1]);
+            for (int i = 0; i < 32; i += 2) tmax = dev::max3(tmax, s[c * 32 + i], s[c * 32 + i + 1]);
           }
           tmax *= scale;
           const bool move = __any_sync(0xffffffffu, tmax > m + (whole == 3 ? 0.f : kMaxSlack));
@@ -539,9 +514,9 @@ __global__ void __launch_bounds__(384, 1)
             if (any >> c & 1) {
 #pragma unroll
               for (int i = c * 32; i < c * 32 + 32; i += 2) {
-                const float2 x = fma2(make_float2(s[i], s[i + 1]), make_float2(scale, scale), make_float2(neg, neg));
+                const float2 x = dev::fma2(make_float2(s[i], s[i + 1]), make_float2(scale, scale), make_float2(neg, neg));
                 const float2 e = make_float2(dev::exp2_approx(x.x), dev::exp2_approx(x.y));
-                sum = add2(sum, e);
+                sum = dev::add2(sum, e);
                 pr[i / 2] = dev::pack2<T>(e.x, e.y);
               }
             } else {
@@ -606,8 +581,8 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           // a row that has seen nothing has zeros there (0 times finite values) or garbage times inv = 0
-          const float2 y = fma2(make_float2(o[2 * i], o[2 * i + 1]), make_float2(inv, inv), make_float2(0.f, 0.f));
-          probe = fma2(y, make_float2(0.f, 0.f), probe);
+          const float2 y = dev::fma2(make_float2(o[2 * i], o[2 * i + 1]), make_float2(inv, inv), make_float2(0.f, 0.f));
+          probe = dev::fma2(y, make_float2(0.f, 0.f), probe);
           v[i] = dev::pack2<T>(y.x, y.y);
         }
         if (live) {

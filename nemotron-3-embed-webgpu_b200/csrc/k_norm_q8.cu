@@ -8,8 +8,10 @@
 //
 // Bound by memory: x, r in, sum and codes out, 7 bytes per element with a
 // residual and 3 without; the row stays in registers between its one read and
-// the writes. W warps (a power of two) share a row, NV 8-column vectors per
-// thread.
+// the writes. wpr warps share a row, NV 8-column vectors per thread. With a
+// dozen scalar operations per element the kernel was bound by instructions (89
+// us at 24000 x 2048, bf16 to e4m3); packed f32 pairs, maxima of three and one
+// division per group brought it to 57, 92 % of the copy rate.
 #include "layer_ops.cuh"
 
 namespace nemo {
@@ -20,17 +22,27 @@ constexpr float kTinyTop = 1e-30f;  // groups no larger than this have codes 0: 
 
 // Up to 8 consecutive elements of a row of n left; elements past them are 0.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
-  if (VEC) {
-    dev::unpack8<T>(*reinterpret_cast<const uint4*>(p), v);
+__device__ __forceinline__ uint4 load8(const T* p, int n) {
+  if constexpr (VEC) {
+    return *reinterpret_cast<const uint4*>(p);
   } else {
+    uint32_t v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? dev::to_f32(p[i]) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + 2 * i;
+      v[i] = (2 * i < n ? h[0] : 0u) | (2 * i + 1 < n ? (uint32_t)h[1] << 16 : 0u);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
   }
 }
 
-template <typename T, int OUT, int NV, bool VEC>
-__global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(const __grid_constant__ NormQ8Args a, int wpr) {
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& u, float2 (&v)[4]) {
+  v[0] = dev::unpack2<T>(u.x), v[1] = dev::unpack2<T>(u.y), v[2] = dev::unpack2<T>(u.z), v[3] = dev::unpack2<T>(u.w);
+}
+
+template <typename T, int OUT, int NV, bool VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS) rmsnorm_q8_kernel(const __grid_constant__ NormQ8Args a, int wpr) {
   __shared__ float red_ss[32];
   __shared__ uint32_t red_top[32];
   constexpr float kQ = OUT == kDtE4M3 ? 448.f : 127.f;
@@ -43,121 +55,153 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(const __grid_constant_
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const T* r = static_cast<const T*>(a.residual) + row * a.ldr;
   T* sum = static_cast<T*>(a.sum) + row * a.lds;
-  float u[NV][8];
-  uint32_t top[NV];
-  float ss = 0.f;
-  uint32_t row_top = 0;
   // every load of the row first
-  float rr[NV][8];
+  uint4 xv[NV], rv[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int c = ((v * wpr + part) * 32 + lane) * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) u[v][i] = rr[v][i] = 0.f;
+    xv[v] = rv[v] = make_uint4(0, 0, 0, 0);
     if (live && c < a.width) {
-      load8<T, VEC>(x + c, a.width - c, u[v]);
-      if (a.residual) load8<T, VEC>(r + c, a.width - c, rr[v]);
+      xv[v] = load8<T, VEC>(x + c, a.width - c);
+      if (a.residual) rv[v] = load8<T, VEC>(r + c, a.width - c);
     }
   }
+  float2 u[NV][4];
+  float top[NV], row_top = 0.f;  // largest |u| of the vector, of the thread; NaN where one is
+  float2 ss2 = make_float2(0.f, 0.f);
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int c = ((v * wpr + part) * 32 + lane) * 8;
-    top[v] = 0;
+    unpack_pairs<T>(xv[v], u[v]);
+    top[v] = 0.f;
     if (live && c < a.width) {
       if (a.residual) {
+        float2 f[4];
+        unpack_pairs<T>(rv[v], f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[v][i] = __fadd_rn(u[v][i], rr[v][i]);
+        for (int i = 0; i < 4; ++i) u[v][i] = dev::add2(u[v][i], f[i]);
+        const uint4 o = make_uint4(dev::pack2<T>(u[v][0].x, u[v][0].y), dev::pack2<T>(u[v][1].x, u[v][1].y),
+                                   dev::pack2<T>(u[v][2].x, u[v][2].y), dev::pack2<T>(u[v][3].x, u[v][3].y));
         if (VEC) {
-          *reinterpret_cast<uint4*>(sum + c) = dev::pack8<T>(u[v]);
+          *reinterpret_cast<uint4*>(sum + c) = o;
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (c + i < a.width) sum[c + i] = dev::from_f32<T>(u[v][i]);
+            if (c + i < a.width) sum[c + i] = dev::from_f32<T>(i & 1 ? u[v][i / 2].y : u[v][i / 2].x);
         }
       }
-      float w[8];
+      float2 w[4];
       if (VEC) {
         const float4 w0 = __ldg(reinterpret_cast<const float4*>(a.w + c));
         const float4 w1 = __ldg(reinterpret_cast<const float4*>(a.w + c) + 1);
-        w[0] = w0.x, w[1] = w0.y, w[2] = w0.z, w[3] = w0.w, w[4] = w1.x, w[5] = w1.y, w[6] = w1.z, w[7] = w1.w;
+        w[0] = make_float2(w0.x, w0.y), w[1] = make_float2(w0.z, w0.w);
+        w[2] = make_float2(w1.x, w1.y), w[3] = make_float2(w1.z, w1.w);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = c + i < a.width ? a.w[c + i] : 0.f;
+        for (int i = 0; i < 4; ++i)
+          w[i] = make_float2(c + 2 * i < a.width ? a.w[c + 2 * i] : 0.f, c + 2 * i + 1 < a.width ? a.w[c + 2 * i + 1] : 0.f);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ss = fmaf(u[v][i], u[v][i], ss);
-        u[v][i] = __fmul_rn(u[v][i], w[i]);
-        // as integers |u| compare like floats, with NaN above infinity
-        top[v] = max(top[v], __float_as_uint(u[v][i]) & 0x7fffffffu);
+      for (int i = 0; i < 4; ++i) {
+        ss2 = dev::fma2(u[v][i], u[v][i], ss2);
+        u[v][i] = dev::mul2(u[v][i], w[i]);
+        top[v] = dev::max3_abs_nan(top[v], u[v][i].x, u[v][i].y);
       }
-      row_top = max(row_top, top[v]);
+      row_top = dev::max3_abs_nan(row_top, top[v], 0.f);
     }
   }
+  float ss = ss2.x + ss2.y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (a.group == 0) row_top = __reduce_max_sync(0xffffffffu, row_top);
+  // as integers magnitudes compare like floats, with NaN above infinity
+  uint32_t row_bits = 0;
+  if (a.group == 0) row_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(row_top));
   if (wpr > 1) {
-    if (lane == 0) red_ss[warp] = ss, red_top[warp] = row_top;
+    if (lane == 0) red_ss[warp] = ss, red_top[warp] = row_bits;
     __syncthreads();
     // every warp of the row sums its parts in the same order
-    ss = 0.f, row_top = 0;
+    ss = 0.f, row_bits = 0;
     for (int i = 0; i < wpr; ++i) {
       ss += red_ss[slot * wpr + i];
-      row_top = max(row_top, red_top[slot * wpr + i]);
+      row_bits = max(row_bits, red_top[slot * wpr + i]);
     }
   }
   const float inv = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)a.width), a.eps));
+  uint32_t bits[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int c = ((v * wpr + part) * 32 + lane) * 8;
-    uint32_t t = row_top;
+    bits[v] = row_bits;
     if (a.group) {
-      t = top[v];
+      uint32_t t = __float_as_uint(top[v]);
       t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
       t = max(t, __shfl_xor_sync(0xffffffffu, t, 2));
       if (a.group >= 64) t = max(t, __shfl_xor_sync(0xffffffffu, t, 4));
       if (a.group >= 128) t = max(t, __shfl_xor_sync(0xffffffffu, t, 8));
+      bits[v] = t;
     }
-    if (!live || c >= a.width) continue;
-    const float tf = __uint_as_float(t);
-    const float to = t < kInfBits && tf > kTinyTop ? __fdiv_rn(kQ, tf) : 0.f;
-    uint8_t code[8];
+  }
+  // The two divisions of a group are made once: lane v of each four (a group
+  // has four lanes or more) makes those of vector v and stores its scale.
+  uint32_t t = bits[0];
+  int vec = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      // an infinity or NaN in the group: codes 0 (its scale below is NaN)
-      const float p0 = t < kInfBits ? __fmul_rn(u[v][i], to) : 0.f;
-      const float p1 = t < kInfBits ? __fmul_rn(u[v][i + 1], to) : 0.f;
+  for (int v = 1; v < NV; ++v)
+    if ((lane & 3) == v) t = bits[v], vec = v;
+  const float tf = __uint_as_float(t);
+  const float to_mine = t < kInfBits && tf > kTinyTop ? __fdiv_rn(kQ, tf) : 0.f;
+  if (live) {
+    const int c = ((vec * wpr + part) * 32 + (lane & ~3)) * 8;  // of the four lanes' first column
+    const bool first = a.group ? c % a.group == 0 : c == 0;
+    if (first && (lane & 3) == vec && c < a.width)
+      a.scales[row * a.groups + (a.group ? c / a.group : 0)] =
+          t < kInfBits ? __fdiv_rn(tf > kTinyTop ? tf * inv : 0.f, kQ) : __uint_as_float(0x7fc00000u);
+  }
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const float to = NV == 1 ? to_mine : __shfl_sync(0xffffffffu, to_mine, (lane & ~3) + v);
+    const int c = ((v * wpr + part) * 32 + lane) * 8;
+    if (!live || c >= a.width) continue;
+    uint2 code;
+    if (bits[v] < kInfBits) {
+      float2 p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = dev::mul2(u[v][i], make_float2(to, to));
       if (OUT == kDtE4M3) {
-        const __nv_fp8x2_storage_t h = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
-        code[i] = (uint8_t)(h & 0xff), code[i + 1] = (uint8_t)(h >> 8);
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __nv_cvt_float2_to_fp8x2(p[i], __NV_SATFINITE, __NV_E4M3);
+        code = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
       } else {
-        code[i] = (uint8_t)min(127, max(-127, __float2int_rn(p0)));
-        code[i + 1] = (uint8_t)min(127, max(-127, __float2int_rn(p1)));
+        // |p| <= 127: adding 1.5 * 2^23 rounds to a whole number, in the low byte
+        // (a scalar addition: the packed one may be merged with the product)
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          h[2 * i] = __float_as_uint(__fadd_rn(p[i].x, 12582912.f));
+          h[2 * i + 1] = __float_as_uint(__fadd_rn(p[i].y, 12582912.f));
+        }
+        code.x = __byte_perm(__byte_perm(h[0], h[1], 0x0040), __byte_perm(h[2], h[3], 0x0040), 0x5410);
+        code.y = __byte_perm(__byte_perm(h[4], h[5], 0x0040), __byte_perm(h[6], h[7], 0x0040), 0x5410);
       }
+    } else {
+      code = make_uint2(0, 0);  // an infinity or NaN in the group, whose scale is NaN
     }
     uint8_t* q = static_cast<uint8_t*>(a.q) + row * a.ldq + c;
     if (VEC) {
-      *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(code);
+      *reinterpret_cast<uint2*>(q) = code;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (c + i < a.width) q[i] = code[i];
-    }
-    // the first thread of each group (of the row for group 0) stores the scale
-    const bool first = a.group ? c % a.group == 0 : c == 0;
-    if (first) {
-      const float scale = t < kInfBits ? __fdiv_rn(tf > kTinyTop ? tf * inv : 0.f, kQ) : __uint_as_float(0x7fc00000u);
-      a.scales[row * a.groups + (a.group ? c / a.group : 0)] = scale;
+        if (c + i < a.width) q[i] = (uint8_t)((i < 4 ? code.x : code.y) >> (i & 3) * 8);
     }
   }
 }
 
 template <typename T, int OUT, bool VEC>
 cudaError_t launch_nv(const NormQ8Args& a, int nv, int wpr, dim3 grid, int threads, cudaStream_t s) {
-  auto kernel = nv == 1   ? rmsnorm_q8_kernel<T, OUT, 1, VEC>
-                : nv == 2 ? rmsnorm_q8_kernel<T, OUT, 2, VEC>
-                          : rmsnorm_q8_kernel<T, OUT, 4, VEC>;
+  auto kernel = nv == 1   ? rmsnorm_q8_kernel<T, OUT, 1, VEC, 512>
+                : nv == 2 ? rmsnorm_q8_kernel<T, OUT, 2, VEC, 512>
+                          : rmsnorm_q8_kernel<T, OUT, 4, VEC, 1024>;
   return launch_overlapped(kernel, grid, dim3(threads), 0, s, dim3(1, 1), a, wpr);
 }
 
@@ -168,14 +212,21 @@ cudaError_t launch_rmsnorm_q8(const NormQ8Args& a, cudaStream_t s) {
   const bool vec = a.width % 8 == 0 && a.ldx % 8 == 0 && aligned(a.x, 16) && aligned(a.w, 16) && a.ldq % 8 == 0 &&
                    aligned(a.q, 8) &&
                    (!a.residual || (a.ldr % 8 == 0 && a.lds % 8 == 0 && aligned(a.residual, 16) && aligned(a.sum, 16)));
-  // One vector per thread while a row fits 32 warps that way.
   const int vectors = (a.width + 7) / 8;
-  int nv = 1, wpr = 1;
-  while (wpr * 32 < vectors && wpr < 32) wpr *= 2;
-  while (nv * wpr * 32 < vectors) nv *= 2;
-  if (nv > 4) return cudaErrorInvalidValue;  // more than 32768 columns
-  const int warps = wpr < 8 ? 8 : wpr;
-  const int64_t rows_per_block = warps / wpr;
+  if (vectors > 4096) return cudaErrorInvalidValue;  // more than 32768 columns
+  // Vectors per thread. Few rows: one, the shortest chain of instructions (one
+  // row of 2048: 2.0 us with one, 3.0 with four; 240 rows 3.2 and 3.6). Rows that
+  // fit a warp: as many as that takes, so that no block barrier is needed (4000
+  // rows of 1000: 5.7 us in one warp, 7.4 in two). Otherwise two, which keeps
+  // enough rows in flight (2400 rows of 2048: 9.0 us, 10.2 with four, 10.9 with
+  // one), and four where the grid is many waves and fewer instructions count
+  // (24000 rows: 58 us with four, 61 with two, 84 with one).
+  const int64_t total = (int64_t)a.rows * vectors;
+  int nv = total <= 148 * 256 ? 1 : vectors <= 128 ? (vectors <= 32 ? 1 : vectors <= 64 ? 2 : 4) : total < 4000000 ? 2 : 4;
+  while (vectors > nv * (nv == 4 ? 1024 : 512)) nv *= 2;
+  const int wpr = (vectors + 32 * nv - 1) / (32 * nv);
+  const int rows_per_block = wpr >= 4 ? 1 : 4 / wpr;
+  const int warps = rows_per_block * wpr;
   const dim3 grid((unsigned)((a.rows + rows_per_block - 1) / rows_per_block));
   const bool e4m3 = a.out_dtype == kDtE4M3;
 #define NEMO_NORM(T)                                                                            \
