@@ -16,12 +16,25 @@
 // segment: the columns that an instruction's k index stands for are permuted,
 // in the same way for the weights and for x, so that each lane reads its
 // weights as one vector and each word's nibble pairs (k, k + 4) come out of
-// one mask; x is stored in shared memory in that order once per block.
+// one mask; x is stored in shared memory in that order.
 //
-// One block owns 16 R rows and a panel of columns; its 8 warps divide the
-// panel, each with its own asynchronous copies, so weights flow without block
-// barriers. Panels of one row tile are blocks of one cluster, summed in rank
-// order through distributed shared memory.
+// A warp's work is 16 R rows and a slice of a panel of columns, in chunks of 256
+// columns (R x 2 KB). Each warp copies its own next chunks and their scales to
+// shared memory while it works on this one, so weights flow without block
+// barriers. The 8 warps of a block are wk slices of 8 / wk row tiles: one slice
+// where there are rows enough for every warp of the GPU, so that nothing is
+// summed over warps; more where there are few rows. Panels (of the columns
+// whose x fits shared memory) of a row tile are blocks of one cluster, summed in
+// rank order through distributed shared memory.
+//
+// Bound: at 6.5 TB/s an SM gets 4 KB of weights (32 rows x 256 columns) in 180
+// cycles, in which its schedulers issue 720 instructions; decoding and
+// multiplying them takes some 450 and the chunk's copies and scales 300. One row
+// of bf16 x against 131072 x 2048: 40 us, 3.5 TB/s (16-row tiles 61, a fixed
+// split of every tile over the 8 warps 51, 64 with the scales read in line and
+// two logic operations a nibble pair); one row against 5120 x 2048: 5.2 us.
+#include <type_traits>
+
 #include "layer_ops.cuh"
 
 namespace nemo {
@@ -31,63 +44,124 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr size_t kSmemLimit = 227 * 1024;
 
+constexpr int kChunk = 256;   // columns of a copy
+constexpr int kPitch = kChunk / 2;
+
 struct W4Plan {
   W4Args a;
-  int segs;         // segments of a row
-  int panel_segs;   // segments of a block's panel
-  int warp_segs;    // segments of a warp's slice of the panel (panel_segs / 8 rounded up)
-  int panels;       // panels of a row
-  int splits;       // blocks per row tile (cluster size)
-  int mp;           // rows of x in shared memory: m rounded up to 1, 2, 4, 8 or 16
-  int w_pitch;      // bytes between weight rows of a warp's slice in shared memory
-  int off_x, off_s, off_xs, off_red;  // byte offsets in shared memory (weights at 0)
+  int segs;        // segments of a row
+  int panel_segs;  // segments of a block's panel
+  int slice_segs;  // segments of a warp's slice of the panel
+  int wk;          // slices of a panel: 1, 2, 4 or 8
+  int panels;      // panels of a row
+  int splits;      // blocks per row tile (cluster size)
+  int tiles;       // block tiles (8 / wk x 16 R rows)
+  int blocks;      // blocks over the tiles
+  int stages;      // chunks in flight
+  int mp;          // rows of x in shared memory: m rounded up to 1, 2, 4, 8 or 16
+  int off_x, off_xs, off_zero, off_red;  // byte offsets in shared memory (the warps' stages at 0)
 };
 
+// A warp's stage: the weights, then the scales of the groups that a chunk can
+// touch (one more where it may start inside a group, which shorter groups of x
+// scales allow).
+template <int SEG, int R>
+struct W4Cfg {
+  static constexpr int kRows = 16 * R;
+  static constexpr int kGroups = kChunk / SEG + (SEG < 128 ? 1 : 0);
+  static constexpr int kStage = kRows * (kPitch + kGroups * 8);
+};
+
+// a & b | c in one instruction (the compiler makes two of constant b and c).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
 // The integers q - z of one 32-bit word as four pairs: (k, k+4), (k+1, k+5),
-// (k+2, k+6), (k+3, k+7). zc = the pair (1024 + z) in f16, (128 + z) in bf16: a
+// (k+2, k+6), (k+3, k+7). zc = the pair -(1024 + z) in f16, -(128 + z) in bf16: a
 // nibble masked under the exponent whose unit is 1 is that base plus q.
 template <typename T>
 struct Nibbles;
 template <>
 struct Nibbles<__half> {
-  static constexpr float kBase = 1024.f;
-  __device__ static __forceinline__ void decode(uint32_t w, uint32_t zc, uint32_t (&p)[4]) {
-    const __half2 z = *reinterpret_cast<const __half2*>(&zc);
-    // high nibbles sit four bits up: 1024 + 16 q, times 1/16 = 64 + q; 64 + z = (1024 + z) - 960
-    const __half2 zh = __hsub2(__floats2half2_rn(960.f, 960.f), z);  // -(64 + z)
-    const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
+  static constexpr uint32_t kBase = 0xe400;  // -1024, whose last bits count ones
+  // high nibbles sit four bits up: 1024 + 16 q, times 1/16 = 64 + q
+  __device__ static __forceinline__ uint32_t high(uint32_t zc) {  // -(64 + z)
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(0x63806380u), "r"(zc));
+    return d;
+  }
+  __device__ static __forceinline__ void decode(uint32_t w, uint32_t zc, uint32_t zh, uint32_t (&p)[4]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t lo = (w & 0x000f000fu) | 0x64006400u, hi = (w & 0x00f000f0u) | 0x64006400u;
-      const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), z);
-      const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, zh);
-      p[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
-      p[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+      const uint32_t lo = and_or(w, 0x000f000fu, 0x64006400u), hi = and_or(w, 0x00f000f0u, 0x64006400u);
+      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(p[2 * i]) : "r"(lo), "r"(zc));
+      asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(p[2 * i + 1]) : "r"(hi), "r"(0x2c002c00u), "r"(zh));
       w >>= 8;
     }
   }
 };
 template <>
 struct Nibbles<__nv_bfloat16> {
-  static constexpr float kBase = 128.f;
-  __device__ static __forceinline__ void decode(uint32_t w, uint32_t zc, uint32_t (&p)[4]) {
-    const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&zc);
+  static constexpr uint32_t kBase = 0xc300;  // -128
+  __device__ static __forceinline__ uint32_t high(uint32_t) { return 0; }
+  __device__ static __forceinline__ void decode(uint32_t w, uint32_t zc, uint32_t, uint32_t (&p)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t v = (w & 0x000f000fu) | 0x43004300u;
-      const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), z);
-      p[i] = *reinterpret_cast<const uint32_t*>(&a);
+      // times 1, plus: one instruction, where a bf16 addition or subtraction takes two
+      asm("fma.rn.bf16x2 %0, %1, %2, %3;"
+          : "=r"(p[i])
+          : "r"(and_or(w, 0x000f000fu, 0x43004300u)), "r"(0x3f803f80u), "r"(zc));
       w >>= 4;
     }
   }
 };
 
-// One element of x as f32 (8-bit codes without their scale).
-__device__ __forceinline__ float load_x(const void* x, int dtype, int64_t i) {
-  if (dtype == kDtF16) return __half2float(static_cast<const __half*>(x)[i]);
-  if (dtype == kDtBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(x)[i]);
-  if (dtype == kDtI8) return (float)static_cast<const int8_t*>(x)[i];
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(x)[i], __NV_E4M3)));
+// Eight elements of x as they lie in memory: 16 bytes of 16-bit ones, 8 of codes.
+template <bool CODES>
+__device__ __forceinline__ uint4 load_x8(const void* x, int64_t at) {
+  if constexpr (CODES) {
+    const uint8_t* p = static_cast<const uint8_t*>(x) + at;
+    uint32_t b[2];
+    if (((uintptr_t)p & 7) == 0) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      b[0] = u.x, b[1] = u.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        b[i] = p[4 * i] | (uint32_t)p[4 * i + 1] << 8 | (uint32_t)p[4 * i + 2] << 16 | (uint32_t)p[4 * i + 3] << 24;
+    }
+    return make_uint4(b[0], b[1], 0, 0);
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(x) + at;
+    if (((uintptr_t)p & 15) == 0) return *reinterpret_cast<const uint4*>(p);
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+// The same in the type of the products (codes without their scale, exact in
+// f16), paired as one word's nibbles are: (0, 4), (1, 5), (2, 6), (3, 7).
+template <bool CODES>
+__device__ __forceinline__ uint4 pair_x8(uint4 u, int dtype) {
+  uint32_t v[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (CODES) {
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      const uint32_t two = v[i / 2] >> (i & 1) * 16;
+      if (dtype == kDtE4M3) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffff), __NV_E4M3);
+        v[i] = h.x | (uint32_t)h.y << 16;
+      } else {
+        v[i] = dev::pack2<__half>((float)(int8_t)(two & 0xff), (float)(int8_t)(two >> 8 & 0xff));
+      }
+    }
+  }
+  return make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), __byte_perm(v[1], v[3], 0x5410),
+                    __byte_perm(v[1], v[3], 0x7632));
 }
 
 template <int N>
@@ -107,26 +181,183 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
 // exactly). R: 16-row tiles per block. NT: 8-row tiles of x. XG: x scales per
 // group.
 template <typename T, int SEG, int R, int NT, bool XG>
-__global__ void __launch_bounds__(kThreads) w4_matvec_kernel(const __grid_constant__ W4Plan p) {
+__global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_constant__ W4Plan p) {
   extern __shared__ __align__(128) uint8_t smem[];
+  using C = W4Cfg<SEG, R>;
   constexpr int WPL = SEG / 32;  // words of a row per lane and segment
-  constexpr int ROWS = 16 * R;
+  constexpr int ROWS = C::kRows, COLS = 8 * NT;
+  constexpr int SEG_BYTES = SEG / 2, CHUNK_SEGS = kChunk / SEG;
   const W4Args& a = p.a;
   dev::pdl_launch_dependents();
   dev::pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row0 = blockIdx.x * ROWS, rank = blockIdx.y;
-  const int seg_bytes = SEG / 2;
-  uint8_t* sw = smem + (size_t)warp * ROWS * p.w_pitch;
+  const int rank = blockIdx.y;
+  const int ks = warp % p.wk, wr = warp / p.wk, row_tiles = kWarps / p.wk;
+  const int block_rows = row_tiles * ROWS;
+  uint8_t* stages = smem + warp * p.stages * C::kStage;
   uint8_t* sx = smem + p.off_x;
-  uint32_t* ss = reinterpret_cast<uint32_t*>(smem + p.off_s);
   float* sxs = reinterpret_cast<float*>(smem + p.off_xs);
-  float* red = reinterpret_cast<float*>(smem + p.off_red);
-  const int64_t row_bytes = a.k / 2;
-  const int groups = a.k / a.group, seg_per_group = a.group / SEG;
+  float* red = reinterpret_cast<float*>(smem + p.off_red);  // two buffers of [wk][COLS][block_rows]
+  const int groups = a.k / a.group;
+  const int seg_shift = a.group == SEG ? 0 : a.group == 2 * SEG ? 1 : 2;  // segments of a group, log2
   const int zero_bytes = (groups + 1) / 2;
   const int x_groups = (a.k + a.x_group - 1) / a.x_group;
+  const int64_t row_bytes = a.k / 2;
 
+  // The warp's chunks in order: tiles blockIdx.x, + gridDim.x, ...; of each, the
+  // panels rank, + splits, ... (one, unless a row has more panels than a cluster
+  // has blocks); of each panel, its slice.
+  struct Cursor {
+    int tile, panel;
+    int seg, left;  // the chunk's first segment, segments of the slice from there on
+  };
+  auto enter = [&](Cursor& c) {  // the slice of c's tile and panel
+    c.seg = c.panel * p.panel_segs + ks * p.slice_segs;
+    c.left = max(0, min(min(p.slice_segs, p.panel_segs - ks * p.slice_segs), p.segs - c.seg));
+  };
+  // To the next chunk; whether that is of another slice. A slice counts as one
+  // chunk at least, so that every warp meets every tile.
+  auto advance = [&](Cursor& c) {
+    c.seg += CHUNK_SEGS, c.left -= CHUNK_SEGS;
+    if (c.left > 0) return false;
+    c.panel += p.splits;
+    if (c.panel >= p.panels) {
+      c.panel = rank;
+      c.tile += gridDim.x;
+    }
+    enter(c);
+    return true;
+  };
+  Cursor next{(int)blockIdx.x, rank, 0, 0}, cur = next;  // to copy, to work on
+  enter(next);
+  enter(cur);
+
+  // The copies. Lane: 16-byte unit lane % 8 of the rows lane / 8 + 4 i of the
+  // weights, at unit u ^ (row % (8 / WPL)) * WPL of its row, so that the lanes'
+  // reads meet no bank twice; the scales and zero points of row lane % ROWS. Rows
+  // past the last one repeat it; their sums are not stored.
+  const int unit = lane & 7, r0 = lane >> 3, own_row = lane % ROWS;
+  const uint8_t* w_from = nullptr;    // the lane's unit of the chunk's first four rows
+  const uint16_t* s_from = nullptr;   // the lane's row of scales
+  const uint8_t* z_from = nullptr;    // and of zero points
+  bool whole = true;                  // every row exists
+  auto aim = [&]() {                  // at the slice of `next`
+    const int row0 = next.tile * block_rows + wr * ROWS;
+    whole = row0 + ROWS <= a.n;
+    w_from = a.w + (int64_t)(row0 + r0) * row_bytes + (int64_t)next.seg * SEG_BYTES + unit * 16;
+    const int64_t row = min(row0 + own_row, a.n - 1);
+    s_from = a.scales + row * groups;
+    z_from = a.zeros + row * zero_bytes;
+  };
+  auto load = [&](int stage) {
+    if (next.tile < p.tiles && unit < next.left * (SEG_BYTES / 16)) {
+      const uint32_t to = dev::smem_u32(stages) + stage * C::kStage + r0 * kPitch;
+      const uint8_t* from = w_from;
+#pragma unroll
+      for (int i = 0; i < ROWS / 4; ++i) {
+        if (!whole) {
+          const int row0 = next.tile * block_rows + wr * ROWS;
+          from = w_from + (int64_t)(min(row0 + i * 4 + r0, a.n - 1) - row0 - r0) * row_bytes;
+        }
+        dev::cp_async16(to + i * 4 * kPitch + (unit ^ ((i * 4 + r0) % (8 / WPL) * WPL)) * 16, from);
+        from += 4 * row_bytes;
+      }
+    }
+    dev::cp_async_commit();
+  };
+  // Scales and zero points are read into registers before the work on another
+  // chunk and put into shared memory after it, as [group][row] of the scale
+  // (f32) and the pair of the zero constant.
+  constexpr int kScales = (C::kGroups + 32 / ROWS - 1) / (32 / ROWS);
+  uint32_t scale16[kScales], zero4[kScales];
+  auto read_scales = [&]() {
+    if (next.tile >= p.tiles) return;
+    const int g0 = next.seg >> seg_shift, n = min(next.left, CHUNK_SEGS);
+    const int ng = n > 0 ? ((next.seg + n - 1) >> seg_shift) - g0 + 1 : 0;
+#pragma unroll
+    for (int j = 0; j < kScales; ++j) {
+      const int i = lane / ROWS + j * (32 / ROWS);
+      scale16[j] = 0, zero4[j] = 8;
+      if (i < ng) {
+        scale16[j] = s_from[g0 + i];
+        if (a.zeros) zero4[j] = (uint32_t)z_from[(g0 + i) >> 1] >> ((g0 + i) & 1) * 4;
+      }
+    }
+  };
+  auto put_scales = [&](int stage) {
+    uint2* ss = reinterpret_cast<uint2*>(stages + stage * C::kStage + ROWS * kPitch);
+#pragma unroll
+    for (int j = 0; j < kScales; ++j) {
+      const int i = lane / ROWS + j * (32 / ROWS);
+      const uint16_t bits = (uint16_t)scale16[j];
+      const float f = a.scale_dtype == kDtBF16 ? __uint_as_float(scale16[j] << 16)
+                                               : __half2float(*reinterpret_cast<const __half*>(&bits));
+      if (i < C::kGroups)
+        ss[i * ROWS + own_row] = make_uint2(__float_as_uint(f), (Nibbles<T>::kBase + (zero4[j] & 15)) * 0x10001u);
+    }
+  };
+  // x of a panel in the order of the instructions: for each 32-column step of a
+  // segment, row of x and lane t, the 8 columns of that lane's word
+  auto load_x = [&](int panel, auto codes) {
+    constexpr bool CODES = decltype(codes)::value;
+    const int seg0 = panel * p.panel_segs, n = min(p.panel_segs, p.segs - seg0);
+    const int units = n * (SEG / 8);  // of a row
+    constexpr int kAhead = 4;         // loads in flight
+    for (int i0 = threadIdx.x; i0 < p.mp * units; i0 += kAhead * kThreads) {
+      uint4 raw[kAhead];
+      int to[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = i0 + j * kThreads;
+        const int m = i / units, u = i - m * units;
+        const int seg = u / (SEG / 8), rem = u % (SEG / 8);
+        to[j] = i < p.mp * units ? (((seg * WPL + rem % WPL) * p.mp + m) * 4 + rem / WPL) * 16 : -1;
+        raw[j] = make_uint4(0, 0, 0, 0);
+        if (m < a.m && i < p.mp * units) raw[j] = load_x8<CODES>(a.x, m * a.ldx + (int64_t)seg0 * SEG + u * 8);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (to[j] >= 0) *reinterpret_cast<uint4*>(sx + to[j]) = pair_x8<CODES>(raw[j], a.x_dtype);
+    }
+    if (XG)
+      for (int i = threadIdx.x; i < n * p.mp; i += kThreads) {
+        const int m = i % p.mp, seg = i / p.mp;
+        sxs[i] = m < a.m ? a.x_scales[(int64_t)m * x_groups + (int64_t)(seg0 + seg) * SEG / a.x_group] : 0.f;
+      }
+  };
+  auto stage_x = [&](int panel) {
+    if (a.x_dtype == kDtE4M3 || a.x_dtype == kDtI8) load_x(panel, std::true_type{});
+    else load_x(panel, std::false_type{});
+  };
+
+
+  const int ahead = p.stages - 1;
+  aim();
+  auto copy = [&](int stage) {  // the next chunk's weights; its scales into registers
+    load(stage);
+    read_scales();
+    w_from += kPitch;
+    if (advance(next)) aim();
+  };
+  for (int i = 0; i < ahead; ++i) {
+    copy(i);
+    put_scales(i);
+  }
+  if (threadIdx.x == 0) *reinterpret_cast<uint4*>(smem + p.off_zero) = make_uint4(0, 0, 0, 0);
+  const bool one_panel = p.panels <= p.splits;
+  if (one_panel) {
+    stage_x(rank);
+    __syncthreads();
+  }
+  // the lane's rows of x; those past the last one read zeros behind it
+  const uint8_t* x_at[NT];
+  int x_step[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const bool live = n * 8 + g < p.mp;
+    x_at[n] = live ? sx + ((n * 8 + g) * 4 + t) * 16 : smem + p.off_zero;
+    x_step[n] = live ? p.mp * 64 : 0;
+  }
   float acc[R][NT][4];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -134,100 +365,61 @@ __global__ void __launch_bounds__(kThreads) w4_matvec_kernel(const __grid_consta
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
-
-  for (int panel = rank; panel < p.panels; panel += p.splits) {
-    const int seg0 = panel * p.panel_segs;
-    const int nseg = min(p.panel_segs, p.segs - seg0);  // of the panel
-    const int ws0 = warp * p.warp_segs;                 // the warp's first segment in the panel
-    const int wn = max(0, min(p.warp_segs, nseg - ws0));
-    // the warp's weights: rows past n repeat the last one (their sums are not stored)
-    const int units = wn * seg_bytes / 16;
-    for (int u0 = 0; u0 < units; u0 += 8) {
-      const int u = u0 + (lane & 7);
-#pragma unroll
-      for (int i = 0; i < ROWS / 4; ++i) {
-        const int row = i * 4 + (lane >> 3);
-        if (u < units)
-          dev::cp_async16(dev::smem_u32(sw + row * p.w_pitch + u * 16),
-                          a.w + (int64_t)min(row0 + row, a.n - 1) * row_bytes + (int64_t)(seg0 + ws0) * seg_bytes + u * 16);
-      }
+  int stage = 0, fill = ahead;  // of this chunk, of the next copy
+  int turn = 0;                 // tiles done
+  while (cur.tile < p.tiles) {
+    copy(fill);
+    if (!one_panel && cur.seg == cur.panel * p.panel_segs + ks * p.slice_segs) {
+      __syncthreads();  // the last panel's x is done with
+      stage_x(cur.panel);
+      __syncthreads();
     }
-    dev::cp_async_commit();
-    // x in the order of the instructions: for each 32-column step of a segment,
-    // row and lane t, the 8 columns of that lane's word, paired (k, k + 4)
-    for (int m = 0; m < p.mp; ++m)
-      for (int u = threadIdx.x; u < nseg * (SEG / 8); u += kThreads) {
-        const int seg = u / (SEG / 8), rem = u % (SEG / 8);
-        const int64_t at = m * a.ldx + (int64_t)(seg0 + seg) * SEG + rem * 8;
-        float v[8];
+    if (p.stages == 3) dev::cp_async_wait<2>();
+    else dev::cp_async_wait<1>();
+    __syncwarp();
+    const uint8_t* st = stages + stage * C::kStage;
+    const uint2* ss = reinterpret_cast<const uint2*>(st + ROWS * kPitch);
+    const int seg0 = cur.seg, g0 = seg0 >> seg_shift, in_panel = seg0 - cur.panel * p.panel_segs;
+    const int n_segs = cur.left;
+    const uint8_t* wp = st + g * kPitch;  // (rows 8 apart have the same swizzle)
+    const int flip = g % (8 / WPL) * WPL * 16;
+    const uint8_t* xp[NT];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = m < a.m ? load_x(a.x, a.x_dtype, at + i) : 0.f;
-        uint4 o;
-        o.x = dev::pack2<T>(v[0], v[4]);
-        o.y = dev::pack2<T>(v[1], v[5]);
-        o.z = dev::pack2<T>(v[2], v[6]);
-        o.w = dev::pack2<T>(v[3], v[7]);
-        const int step = seg * WPL + rem % WPL, l = rem / WPL;
-        *reinterpret_cast<uint4*>(sx + ((step * p.mp + m) * 4 + l) * 16) = o;
-      }
-    // scale (low half, as stored) and zero constant (high half) of each group and row
-    const int g0 = seg0 / seg_per_group, ng = (nseg + seg_per_group - 1) / seg_per_group;
-    for (int i = threadIdx.x; i < ng * ROWS; i += kThreads) {
-      const int row = i / ng, gr = i - row * ng;
-      const int64_t r = min(row0 + row, a.n - 1);
-      float z = 8.f;
-      if (a.zeros) z = (float)((a.zeros[r * zero_bytes + (g0 + gr) / 2] >> (((g0 + gr) & 1) * 4)) & 15);
-      const uint32_t zc = dev::pack2<T>(0.f, Nibbles<T>::kBase + z);
-      ss[gr * ROWS + row] = zc | a.scales[r * groups + g0 + gr];
-    }
-    if (XG)
-      for (int i = threadIdx.x; i < nseg * p.mp; i += kThreads) {
-        const int m = i % p.mp, seg = i / p.mp;
-        sxs[i] = m < a.m ? a.x_scales[(int64_t)m * x_groups + (seg0 + seg) * SEG / a.x_group] : 0.f;
-      }
-    dev::cp_async_wait<0>();
-    __syncthreads();
-
-    for (int s = 0; s < wn; ++s) {
-      const int seg = ws0 + s, gr = seg / seg_per_group;
-      uint32_t w[R][2][WPL], zc[R][2];
+    for (int n = 0; n < NT; ++n) xp[n] = x_at[n] + in_panel * WPL * x_step[n];
+#pragma unroll
+    for (int s = 0; s < CHUNK_SEGS; ++s) {
+      if (s >= n_segs) break;
+      const uint2* sp = ss + (((seg0 + s) >> seg_shift) - g0) * ROWS + g;
+      uint32_t w[R][2][WPL], zc[R][2], zh[R][2];
       float sc[R][2];
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int row = r * 16 + h * 8 + g;
-          lds_words<WPL>(sw + row * p.w_pitch + s * seg_bytes + t * WPL * 4, w[r][h]);
-          const uint32_t v = ss[gr * ROWS + row];
-          zc[r][h] = __byte_perm(v, v, 0x3232);
-          const uint16_t bits = (uint16_t)v;
-          sc[r][h] = a.scale_dtype == kDtBF16 ? __uint_as_float(v << 16)
-                                              : __half2float(*reinterpret_cast<const __half*>(&bits));
+          lds_words<WPL>(wp + (r * 16 + h * 8) * kPitch + ((s * SEG_BYTES + t * WPL * 4) ^ flip), w[r][h]);
+          const uint2 v = sp[r * 16 + h * 8];
+          sc[r][h] = __uint_as_float(v.x);
+          zc[r][h] = v.y;
+          zh[r][h] = Nibbles<T>::high(v.y);
         }
       float part[R][NT][4];
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) part[r][n][i] = 0.f;
 #pragma unroll
       for (int j = 0; j < WPL; ++j) {
         uint4 b[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          b[n] = make_uint4(0, 0, 0, 0);
-          if (n * 8 + g < p.mp)
-            b[n] = *reinterpret_cast<const uint4*>(sx + (((seg * WPL + j) * p.mp + n * 8 + g) * 4 + t) * 16);
+          b[n] = *reinterpret_cast<const uint4*>(xp[n]);
+          xp[n] += x_step[n];
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           uint32_t lo[4], hi[4];
-          Nibbles<T>::decode(w[r][0][j], zc[r][0], lo);
-          Nibbles<T>::decode(w[r][1][j], zc[r][1], hi);
+          Nibbles<T>::decode(w[r][0][j], zc[r][0], zh[r][0], lo);
+          Nibbles<T>::decode(w[r][1][j], zc[r][1], zh[r][1], hi);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            dev::mma_16816<T>(part[r][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
+            if (j == 0) dev::mma_16816_zero<T>(part[r][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
+            else dev::mma_16816<T>(part[r][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
             dev::mma_16816<T>(part[r][n], lo[2], hi[2], lo[3], hi[3], b[n].z, b[n].w);
           }
         }
@@ -237,8 +429,8 @@ __global__ void __launch_bounds__(kThreads) w4_matvec_kernel(const __grid_consta
         float f0 = 1.f, f1 = 1.f;  // x scales of the lane's two rows of x
         if (XG) {
           const int m = n * 8 + 2 * t;
-          f0 = m < p.mp ? sxs[seg * p.mp + m] : 0.f;
-          f1 = m + 1 < p.mp ? sxs[seg * p.mp + m + 1] : 0.f;
+          f0 = m < p.mp ? sxs[(in_panel + s) * p.mp + m] : 0.f;
+          f1 = m + 1 < p.mp ? sxs[(in_panel + s) * p.mp + m + 1] : 0.f;
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -249,59 +441,59 @@ __global__ void __launch_bounds__(kThreads) w4_matvec_kernel(const __grid_consta
         }
       }
     }
-    __syncthreads();  // before the next panel overwrites shared memory
-  }
+    put_scales(fill);
+    __syncwarp();  // the stage is free for the next copy
+    stage = stage + 1 == p.stages ? 0 : stage + 1;
+    fill = fill + 1 == p.stages ? 0 : fill + 1;
+    const int tile = cur.tile;
+    advance(cur);
+    if (cur.tile == tile) continue;
 
-  // sums over the warps, then over the cluster's panels, both in order
-  constexpr int COLS = 8 * NT;
+    // the tile's sums
+    auto store = [&](int m, int row, float y) {
+      if (!XG && a.x_scales) y *= a.x_scales[m];
+      const int64_t at = m * a.ldy + row;
+      if (a.y_dtype == kDtF32) static_cast<float*>(a.y)[at] = y;
+      else if (a.y_dtype == kDtBF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(y);
+      else static_cast<__half*>(a.y)[at] = __float2half_rn(y);
+    };
+    const bool alone = p.wk == 1 && p.splits == 1;  // no other warp has a part of them
+    float* mine = red + (turn++ & 1) * (p.wk * COLS * block_rows);
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        red[(warp * COLS + n * 8 + 2 * t + (i & 1)) * ROWS + r * 16 + (i >> 1) * 8 + g] = acc[r][n][i];
-  __syncthreads();
-  float* total = red;  // [COLS][ROWS], over warp 0's part
-  constexpr int kEach = (COLS * ROWS + kThreads - 1) / kThreads;
-  float v[kEach];
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = e * kThreads + threadIdx.x;
-    v[e] = 0.f;
-    if (i < a.m * ROWS)
-      for (int w = 0; w < kWarps; ++w) v[e] += red[w * COLS * ROWS + i];
-  }
-  if (p.splits > 1) {
+        for (int i = 0; i < 4; ++i) {
+          const int m = n * 8 + 2 * t + (i & 1), row = wr * ROWS + r * 16 + (i >> 1) * 8 + g;
+          if (m < a.m) {
+            if (!alone) mine[(ks * COLS + m) * block_rows + row] = acc[r][n][i];
+            else if (tile * block_rows + row < a.n) store(m, tile * block_rows + row, acc[r][n][i]);
+          }
+          acc[r][n][i] = 0.f;
+        }
+    if (alone) continue;
+    // over the warps, then over the cluster's panels, both in order; the buffers
+    // alternate, so the next tile's sums need no second barrier
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = e * kThreads + threadIdx.x;
-      if (i < a.m * ROWS) total[i] = v[e];
+    for (int i = threadIdx.x; i < a.m * block_rows; i += kThreads) {
+      float v = 0.f;
+      for (int w = 0; w < p.wk; ++w) v += mine[w * COLS * block_rows + i];
+      if (p.splits > 1) mine[i] = v;  // [COLS][block_rows], over slice 0's part
+      else if (tile * block_rows + i % block_rows < a.n) store(i / block_rows, tile * block_rows + i % block_rows, v);
     }
-    dev::cluster_sync();
-    if (rank == 0) {
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int i = e * kThreads + threadIdx.x;
-        if (i < a.m * ROWS)
-          for (int c = 1; c < p.splits; ++c) v[e] += dev::ld_dsmem_f32(dev::mapa(dev::smem_u32(total + i), c));
-      }
+    if (p.splits > 1) {
+      dev::cluster_sync();
+      if (rank == 0)
+        for (int i = threadIdx.x; i < a.m * block_rows; i += kThreads) {
+          float v = mine[i];
+          for (int c = 1; c < p.splits; ++c) v += dev::ld_dsmem_f32(dev::mapa(dev::smem_u32(mine + i), c));
+          if (tile * block_rows + i % block_rows < a.n) store(i / block_rows, tile * block_rows + i % block_rows, v);
+        }
     }
-    dev::cluster_sync();  // no block leaves while its sums are read
-    if (rank) return;
   }
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = e * kThreads + threadIdx.x;
-    const int m = i / ROWS, row = row0 + i % ROWS;
-    if (i >= a.m * ROWS || row >= a.n) continue;
-    const float y = !XG && a.x_scales ? v[e] * a.x_scales[m] : v[e];
-    const int64_t at = m * a.ldy + row;
-    if (a.y_dtype == kDtF32) static_cast<float*>(a.y)[at] = y;
-    else if (a.y_dtype == kDtBF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(y);
-    else static_cast<__half*>(a.y)[at] = __float2half_rn(y);
-  }
+  dev::cp_async_wait<0>();
+  if (p.splits > 1) dev::cluster_sync();  // no block leaves while its sums are read
 }
 
 template <typename T, int SEG, int R, int NT, bool XG>
@@ -317,7 +509,7 @@ cudaError_t launch_kernel(const W4Plan& p, size_t smem, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  const dim3 grid((unsigned)((p.a.n + 16 * R - 1) / (16 * R)), (unsigned)p.splits);
+  const dim3 grid((unsigned)p.blocks, (unsigned)p.splits);
   return launch_overlapped(kernel, grid, dim3(kThreads), smem, s, dim3(1, p.splits), p);
 }
 
@@ -347,32 +539,50 @@ cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s) {
   p.segs = a.k / seg;
   p.mp = a.m <= 1 ? 1 : a.m <= 2 ? 2 : a.m <= 4 ? 4 : a.m <= 8 ? 8 : 16;
   const int nt = p.mp == 16 ? 2 : 1;
-  const int r = a.n >= 32 * 148 ? 2 : 1;
-  const int rows = 16 * r;
-  // A panel's weights and rows of x take at most 64 KB of shared memory each;
-  // a multiple of the weight group, so that no group is split.
-  int panel_k = 64 * 1024 * 2 / rows;
-  if (panel_k > 64 * 1024 / 2 / p.mp) panel_k = 64 * 1024 / 2 / p.mp;
-  panel_k = panel_k < a.k ? panel_k / a.group * a.group : a.k;
+  // A panel's rows of x take at most 48 KB of shared memory; a multiple of the
+  // weight group, so that no group is split over panels.
+  int panel_k = 48 * 1024 / 2 / p.mp;
+  int panels = (a.k + panel_k - 1) / panel_k;
+  panel_k = ((a.k + panels - 1) / panels + a.group - 1) / a.group * a.group;  // panels of one length
   p.panels = (a.k + panel_k - 1) / panel_k;
   p.splits = p.panels < 8 ? p.panels : 8;
-  panel_k = ((a.k + p.panels - 1) / p.panels + a.group - 1) / a.group * a.group;  // panels of one length
-  p.panels = (a.k + panel_k - 1) / panel_k;
-  p.splits = p.panels < p.splits ? p.panels : p.splits;
   p.panel_segs = panel_k / seg;
-  p.warp_segs = (p.panel_segs + kWarps - 1) / kWarps;
-  const int slice = p.warp_segs * seg / 2;
-  p.w_pitch = (slice + 127) / 128 * 128 + 16 * (seg / 32);
-  size_t off = (size_t)kWarps * rows * p.w_pitch;
-  p.off_x = (int)off;
-  off += (size_t)p.mp * panel_k * 2;
-  p.off_s = (int)off;
-  off += (size_t)(panel_k / a.group) * rows * 4;
-  p.off_xs = (int)off;
-  if (xg) off += (size_t)p.panel_segs * p.mp * 4;
-  p.off_red = (int)((off + 15) / 16 * 16);
-  off = p.off_red + (size_t)kWarps * 8 * nt * rows * 4;
-  if (off > kSmemLimit) return cudaErrorInvalidValue;
+  auto smem_of = [&](int r, int stages) {
+    const int stage_bytes = 16 * r * (kPitch + (kChunk / seg + (seg < 128 ? 1 : 0)) * 8);
+    size_t off = (size_t)kWarps * stages * stage_bytes;
+    p.off_x = (int)((off + 127) / 128 * 128);
+    off = p.off_x + (size_t)p.mp * panel_k * 2;
+    p.off_xs = (int)off;
+    if (xg) off += (size_t)p.panel_segs * p.mp * 4;
+    p.off_zero = (int)((off + 15) / 16 * 16);
+    p.off_red = p.off_zero + 16;
+    return p.off_red + (size_t)2 * kWarps * 8 * nt * 16 * r * 4;
+  };
+  // The shape (16 or 32 rows a warp, slices of a panel) with the least modelled
+  // time: rounds of blocks over the SMs, times the chunks of a slice (16 rows
+  // take 0.6 of the time of 32) plus a tile's sums (a third of a chunk; two
+  // chunks with a cluster's barriers).
+  double best = 0;
+  int r = 0;
+  for (int rr = 1; rr <= 2; ++rr) {
+    // three stages where two blocks still fit an SM, or two
+    const int stages = smem_of(rr, 3) <= kSmemLimit / 2 ? 3 : 2;
+    const size_t bytes = smem_of(rr, stages);
+    if (bytes > kSmemLimit) continue;
+    const int resident = (bytes <= kSmemLimit / 2 ? 2 : 1) * 148 / p.splits;
+    for (int wk = 1; wk <= 8; wk *= 2) {
+      const int64_t block_rows = 16LL * rr * (8 / wk), tiles = (a.n + block_rows - 1) / block_rows;
+      const int slice = (p.panel_segs + wk - 1) / wk, chunks = (slice * seg + kChunk - 1) / kChunk;
+      const double cost = (double)((tiles + resident - 1) / resident) *
+                          (chunks * (rr == 1 ? 0.6 : 1.0) + (p.splits > 1 ? 2.0 : 0.35));
+      if (r && cost >= best) continue;
+      best = cost, r = rr;
+      p.wk = wk, p.slice_segs = slice, p.tiles = (int)tiles, p.stages = stages;
+      p.blocks = p.tiles < resident ? p.tiles : resident;
+    }
+  }
+  if (!r) return cudaErrorInvalidValue;
+  const size_t off = smem_of(r, p.stages);
   return a.x_dtype == kDtBF16 ? launch_seg<__nv_bfloat16>(p, seg, r, xg, off, s) : launch_seg<__half>(p, seg, r, xg, off, s);
 }
 
