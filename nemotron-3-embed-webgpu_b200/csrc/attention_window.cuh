@@ -9,6 +9,8 @@ namespace nemo {
 
 // 16 rows of one kv head's group per tile (k_attention_rows.cu).
 cudaError_t launch_attention_rows(const AttnWindowArgs& a, cudaStream_t s);
+// Keys that `rows` consecutive queries see, at most.
+int64_t visible_keys(const AttnWindowArgs& a, int rows);
 
 // Request b with its offsets clamped into the buffers, so that a wrong offset
 // cannot make a kernel leave them.

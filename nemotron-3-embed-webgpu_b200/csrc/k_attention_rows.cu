@@ -21,18 +21,22 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kChunk = 32;  // keys per copy
+constexpr int kChunk = 16;  // keys per copy
+constexpr int kMaxSplits = 16;
 
 template <int D, int STAGES>
 struct RowsCfg {
   static constexpr int kRowBytes = D * 2;
   static constexpr int kStage = 2 * kChunk * kRowBytes;  // K, then V
   static constexpr int kRing = kWarps * STAGES * kStage;
-  // the merge reuses the ring: [warp][16][D] f32, then [warp][16] max and sum;
-  // the block's own [16][D], [16], [16] lie behind it
-  static constexpr int kMerge = kWarps * 16 * (D + 2) * 4;
-  static constexpr int kBlock = 16 * (D + 2) * 4;
-  static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kBlock + 64;
+  // the warps' partial results reuse the ring: [warp][16][D] f32
+  static constexpr int kMerge = kWarps * 16 * D * 4;
+  static constexpr int kArea = kRing > kMerge ? kRing : kMerge;
+  // behind it: maximum and sum of [warp][16], then what the cluster's blocks send:
+  // of each rank 16 rows of this block's columns, maximum and sum of 16 rows
+  static constexpr int kStats = 2 * kWarps * 16 * 4;
+  static constexpr int kSent = 16 * D * 4 + 2 * kMaxSplits * 16 * 4;
+  static constexpr int kSmem = kArea + kStats + kSent + 64;
 };
 
 template <typename T, int D, int STAGES>
@@ -41,6 +45,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
   using C = RowsCfg<D, STAGES>;
   extern __shared__ __align__(1024) uint8_t smem[];
   dev::pdl_launch_dependents();
+  if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this block has started
   dev::pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
@@ -49,7 +54,10 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
   const int group = a.q_heads / a.kv_heads;
   const int nq = min(rq.nq, a.max_q);
   const int rows = nq * group;  // of this request and kv head
-  if (tile * 16 >= rows) return;  // the whole cluster
+  if (tile * 16 >= rows) {  // the whole cluster
+    if (splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    return;
+  }
   const int i_first = tile * 16 / group, i_last = min(tile * 16 + 15, rows - 1) / group;
   const int p_off = rq.nk - rq.nq;  // position of query 0
   const KeyRange range(a, i_first + p_off, i_last + p_off, rq.nk);
@@ -126,9 +134,9 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
     const uint32_t sk = dev::smem_u32(ring + (it % STAGES) * C::kStage), sv = sk + kChunk * C::kRowBytes;
     int base, end;
     chunk_keys(c, base, end);
-    float s[4][4];
+    float s[kChunk / 8][4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+    for (int n = 0; n < kChunk / 8; ++n) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
       const int key = n * 8 + (lane & 7);
@@ -141,7 +149,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
       }
     }
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int n = 0; n < kChunk / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = base + n * 8 + 2 * t + (i & 1);
@@ -152,7 +160,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
     for (int h = 0; h < 2; ++h) {
       float mx = m[h];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+      for (int n = 0; n < kChunk / 8; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen yet: all weights 0
@@ -160,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
       m[h] = mx;
       float sum = 0.f;
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < kChunk / 8; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float w = dev::exp2_approx(s[n][2 * h + i] - ref);
@@ -175,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
       o[n][2] *= keep[1], o[n][3] *= keep[1];
     }
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
+    for (int ks = 0; ks < kChunk / 16; ++ks) {
       const uint32_t p0 = dev::pack2<T>(s[2 * ks][0], s[2 * ks][1]), p1 = dev::pack2<T>(s[2 * ks][2], s[2 * ks][3]);
       const uint32_t p2 = dev::pack2<T>(s[2 * ks + 1][0], s[2 * ks + 1][1]),
                      p3 = dev::pack2<T>(s[2 * ks + 1][2], s[2 * ks + 1][3]);
@@ -193,13 +201,14 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
   dev::cp_async_wait<0>();
   __syncthreads();  // the ring becomes the merge buffer
 
-  float* mo = reinterpret_cast<float*>(smem);  // [warp][16][D]
-  float* mm = mo + kWarps * 16 * D;            // [warp][16]
+  float* mo = reinterpret_cast<float*>(smem);             // [warp][16][D]
+  float* mm = reinterpret_cast<float*>(smem + C::kArea);  // [warp][16]
   float* ml = mm + kWarps * 16;
-  float* bo = reinterpret_cast<float*>(smem + (C::kRing > C::kMerge ? C::kRing : C::kMerge));  // [16][D]
-  float* bm = bo + 16 * D;
-  float* bl = bm + 16;
-  uint32_t* bad = reinterpret_cast<uint32_t*>(bl + 16);  // rows with a result that is not finite
+  const int width = D / splits;                           // columns that this block writes
+  float* so = ml + kWarps * 16;                           // sent: [rank][16][width]
+  float* sm = so + 16 * D;                                // [rank][16]
+  float* sl = sm + kMaxSplits * 16;
+  uint32_t* bad = reinterpret_cast<uint32_t*>(sl + kMaxSplits * 16);  // rows with a result that is not finite
   if (threadIdx.x == 0) *bad = 0;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -212,51 +221,71 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
           make_float2(o[n][2 * h], o[n][2 * h + 1]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * D; i += kThreads) {
-    const int row = i / D;
-    float mx = -INFINITY;
+  // Every other block of the cluster runs by now, so its shared memory may be written.
+  if (splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  // The block's result: a thread has 16 / 4 rows of one column group of four. It
+  // goes to the block that writes these columns (maximum and sum to all).
+  constexpr int kQuads = D / 4, kStep = kThreads / kQuads;
+  const int quad = threadIdx.x % kQuads, col = quad * 4, owner = col / width;
+  const uint32_t to_o = dev::smem_u32(so) + (rank * 16 * width + col - owner * width) * 4;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, mm[w * 16 + row]);
+  for (int i = 0; i < 16 / kStep; ++i) {
+    const int row = i * kStep + threadIdx.x / kQuads;
+    float mw[kWarps], mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, mw[w] = mm[w * 16 + row]);
     const float ref = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f, acc = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2f(mm[w * 16 + row] - ref);
+      const float f = dev::exp2_approx(mw[w] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(mo + (w * 16 + row) * D + col);
       sum += ml[w * 16 + row] * f;
-      acc += mo[w * 16 * D + i] * f;
+      acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
     }
-    bo[i] = acc;
-    if (i % D == 0) bm[row] = mx, bl[row] = sum;
-  }
-  // this rank's columns [d0, d1) of every row
-  const int d0 = rank * (D / splits), d1 = d0 + D / splits, width = D / splits;
-  if (splits > 1) dev::cluster_sync();
-  else __syncthreads();
-  for (int i = threadIdx.x; i < 16 * width; i += kThreads) {
-    const int row = i / width, col = d0 + i % width;
-    const int global_row = tile * 16 + row;
-    float acc, sum;
     if (splits > 1) {
-      float mx = -INFINITY;
-      for (int c = 0; c < splits; ++c) mx = fmaxf(mx, dev::ld_dsmem_f32(dev::mapa(dev::smem_u32(bm + row), c)));
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      acc = sum = 0.f;
-      for (int c = 0; c < splits; ++c) {
-        const float f = exp2f(dev::ld_dsmem_f32(dev::mapa(dev::smem_u32(bm + row), c)) - ref);
-        sum += dev::ld_dsmem_f32(dev::mapa(dev::smem_u32(bl + row), c)) * f;
-        acc += dev::ld_dsmem_f32(dev::mapa(dev::smem_u32(bo + row * D + col), c)) * f;
+      const uint32_t at = dev::mapa(to_o + row * width * 4, owner);
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(acc.x), "f"(acc.y), "f"(acc.z),
+                   "f"(acc.w)
+                   : "memory");
+      if (quad < splits) {
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dev::mapa(dev::smem_u32(sm + rank * 16 + row), quad)), "f"(mx)
+                     : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dev::mapa(dev::smem_u32(sl + rank * 16 + row), quad)), "f"(sum)
+                     : "memory");
       }
     } else {
-      acc = bo[row * D + col], sum = bl[row];
+      *reinterpret_cast<float4*>(so + row * D + col) = acc;
+      if (quad == 0) sm[row] = mx, sl[row] = sum;
+    }
+  }
+  if (splits > 1) dev::cluster_sync();
+  else __syncthreads();
+  // this rank's columns [d0, d1) of every row, over the ranks in order
+  const int d0 = rank * width, d1 = d0 + width;
+  for (int i = threadIdx.x; i < 16 * width / 4; i += kThreads) {
+    const int row = i / (width / 4), c = i % (width / 4) * 4;
+    const int global_row = tile * 16 + row;
+    float mx = -INFINITY, sum = 0.f;
+    for (int k = 0; k < splits; ++k) mx = fmaxf(mx, sm[k * 16 + row]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < splits; ++k) {
+      const float f = dev::exp2_approx(sm[k * 16 + row] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(so + (k * 16 + row) * width + c);
+      sum += sl[k * 16 + row] * f;
+      acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
     }
     if (global_row >= rows) continue;
-    const float y = sum == 0.f ? 0.f : acc / sum;
-    if (!isfinite(y)) atomicOr(bad, 1u << row);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+    if (!isfinite(acc.x + acc.y + acc.z + acc.w)) atomicOr(bad, 1u << row);
     const int qi = global_row / group, head = kvh * group + global_row % group;
-    static_cast<T*>(a.out)[(int64_t)(rq.q0 + qi) * a.ldo + head * D + col] = dev::from_f32<T>(y);
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(rq.q0 + qi) * a.ldo + head * D + d0 + c) =
+        make_uint2(dev::pack2<T>(acc.x, acc.y), dev::pack2<T>(acc.z, acc.w));
   }
-  if (splits > 1) dev::cluster_sync();  // no block leaves while its partial results are read
-  else __syncthreads();
+  __syncthreads();
   uint32_t rest = *bad;
   for (int n = 0; rest; ++n, rest &= rest - 1) {
     const int row = __ffs(rest) - 1, global_row = tile * 16 + row;
@@ -277,22 +306,23 @@ cudaError_t launch_rows(const AttnWindowArgs& a, cudaStream_t s) {
   if (dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
   const int group = a.q_heads / a.kv_heads;
   const int64_t tiles = ((int64_t)a.max_q * group + 15) / 16;
-  // keys that a tile's queries see, at most
-  int64_t keys = a.max_k;
-  if (a.left >= 0) {
-    const int64_t window = (int64_t)a.left + (a.right > 0 ? a.right : a.right < 0 ? a.max_k : 0) + 16 + a.sinks;
-    if (window < keys) keys = window;
-  }
+  const int64_t keys = visible_keys(a, 16);
   const int64_t chunks = (keys + kChunk - 1) / kChunk;
-  // split the keys while there are fewer blocks than SMs and every warp keeps
-  // two chunks
+  // Split the keys over a cluster while two blocks an SM are not reached and
+  // every warp keeps two chunks (16 tokens on 1028 keys: 16.3 us with two blocks
+  // a tile, 24.9 with one); beyond that, up to eight, while it keeps 32, which
+  // levels ragged lengths (16 tokens on up to 32768 keys: 193 us, 256 without).
   int splits = 1;
-  while (splits < 8 && tiles * a.kv_heads * a.batch * splits * 2 <= 148 && chunks >= splits * 2 * kWarps * 2) splits *= 2;
+  const int64_t blocks = tiles * a.kv_heads * a.batch;
+  while (splits < kMaxSplits && chunks >= splits * 2 * kWarps * 2 &&
+         (blocks * splits * 2 <= 296 || (blocks * splits * 2 <= 8 * 148 && chunks >= splits * 2 * kWarps * 32)))
+    splits *= 2;
   const dim3 grid((unsigned)(tiles * splits), a.kv_heads, a.batch);
   return launch_overlapped(kernel, grid, dim3(kThreads), C::kSmem, s, dim3(splits, 1), a, splits, (int)tiles);
 }

@@ -201,8 +201,10 @@ WINDOWS = [(-1, -1, 0), (-1, 0, 0), (0, 0, 0), (5, 0, 3), (40, 17, 1), (200, 0, 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("window", WINDOWS, ids=lambda w: "l%d_r%d_s%d" % w)
 @pytest.mark.parametrize("qs,ks", [([1], [1]), ([1, 1, 1], [1, 700, 33]), ([3], [3]), ([17, 0, 2, 40], [17, 9, 64, 40]),
-                                   ([130, 1], [130, 300]), ([300, 257], [300, 600]), ([20, 4], [7, 0])],
-                         ids=["1", "tokens", "3", "ragged", "130", "long", "fewer_keys"])
+                                   ([130, 1], [130, 300]), ([300, 257], [300, 600]), ([20, 4], [7, 0]),
+                                   ([1400, 0, 513, 1], [1400, 5, 901, 1]), ([1300, 700], [90, 0])],
+                         ids=["1", "tokens", "3", "ragged", "130", "long", "fewer_keys", "documents",
+                              "documents_fewer_keys"])
 def test_attention_window(gen, dt, d, window, qs, ks):
     hq, hk = (6, 2) if d == 128 else (5, 1)
     args = packed(gen, dt, qs, ks, hq, hk, d)
@@ -212,7 +214,7 @@ def test_attention_window(gen, dt, d, window, qs, ks):
 
 @pytest.mark.parametrize("hq,hk", [(1, 1), (8, 8), (24, 8), (32, 2), (40, 1)])
 def test_attention_window_head_layouts(gen, hq, hk):
-    for qs, ks in (([2, 1], [900, 5000]), ([150], [333])):
+    for qs, ks in (([2, 1], [900, 5000]), ([150], [333]), ([1100, 700], [1300, 700])):
         args = packed(gen, F16, qs, ks, hq, hk, 128)
         got = ref.attention(*args, 257, 0, 4)
         ref.check_attention(*args, 257, 0, 4, got)
@@ -229,7 +231,7 @@ def test_attention_window_cache_with_room_and_untouched_rows(gen):
     """Keys in a cache [request][capacity] whose unused rows hold NaN, inside a QKV-like row stride; rows of q and out
     behind the last request stay as they were."""
     cap, hq, hk, d = 700, 6, 2, 128
-    for q_len, lens in ((1, [0, 1, 333, 700]), (90, [90, 130, 333, 700])):
+    for q_len, lens in ((1, [0, 1, 333, 700]), (90, [90, 130, 333, 700]), (600, [600, 611, 677, 700])):
         cache = torch.full((4 * cap, 3 * hk * d), float("nan"), dtype=torch.float16, device="cuda")
         for b, n in enumerate(lens):
             cache[b * cap:b * cap + n] = normal(gen, n, 3 * hk * d, dt=F16)
@@ -246,10 +248,10 @@ def test_attention_window_cache_with_room_and_untouched_rows(gen):
 
 
 @TYPES
-@pytest.mark.parametrize("q_len", [1, 4, 70, 300])
-def test_attention_window_garbage_in_unseen_keys(gen, dt, q_len):
+@pytest.mark.parametrize("q_len,nk", [(1, 420), (4, 420), (70, 420), (300, 420), (3000, 3200)])
+def test_attention_window_garbage_in_unseen_keys(gen, dt, q_len, nk):
     """Infinities and NaN in keys and values reach the rows that see them, as NaN or infinity, and no other row."""
-    nk, hq, hk, d = 420, 4, 2, 64
+    hq, hk, d = 4, 2, 64
     args = packed(gen, dt, [q_len], [nk], hq, hk, d)
     q, k, v = args[:3]
     clean = [t.clone() for t in (k, v)]
@@ -295,15 +297,15 @@ def test_attention_window_bad_keys_in_the_open(gen, dt, q_len, bad):
         ref.check_attention(*one, -1, -1, 0, got[:, 64:])
 
 
-@pytest.mark.parametrize("q_len", [1, 200])
-def test_attention_window_large_scores(gen, q_len):
+@pytest.mark.parametrize("q_len,hq", [(1, 2), (200, 2), (900, 8)])
+def test_attention_window_large_scores(gen, q_len, hq):
     """Scores of several thousand: the largest key takes all the weight, nothing overflows."""
-    args = packed(gen, F16, [q_len], [500], 2, 1, 128)
+    args = packed(gen, F16, [q_len], [500 if q_len < 500 else 1200], hq, 1, 128)
     args[0].mul_(30), args[1].mul_(30)
     got = ref.attention(*args, -1, -1, 0, scale=1.0)
     # scores reach 2^17, where an f32 sum of 128 products is good to about 2^-6: compare with the best key where it
     # leads by more
-    s = torch.einsum("qhd,khd->hqk", args[0].double(), args[1].double().expand(-1, 2, -1))
+    s = torch.einsum("qhd,khd->hqk", args[0].double(), args[1].double().expand(-1, hq, -1))
     top = s.topk(2, -1)
     clear = (top.values[..., 0] - top.values[..., 1]) > 20
     assert clear.any()
@@ -311,7 +313,7 @@ def test_attention_window_large_scores(gen, q_len):
     ref.close(got.permute(1, 0, 2)[clear], want[clear], 2.0 ** -10 * want[clear].abs() + 2.0 ** -16)
 
 
-@pytest.mark.parametrize("q_len", [1, 130])
+@pytest.mark.parametrize("q_len", [1, 130, 800])
 def test_attention_window_offsets_past_32_bits(q_len):
     """A cache whose later rows lie more than 2^32 bytes in."""
     rows, hk, d = 1_300_000, 8, 128
@@ -334,10 +336,10 @@ def test_repeats_streams_and_graphs_give_the_same_bits(gen):
     x, r, w = normal(gen, 50, 2048, dt=F16), normal(gen, 50, 2048, dt=F16), normal(gen, 2048)
     wx, xs, wq, s, z = w4_inputs(gen, E4M3, 3, 1024, 4096, 64, True, F16, 128)
     w4, z4 = ref.pack4(wq), ref.pack4(z)
-    q, k, v = (normal(gen, n, 8, 128, dt=F16) for n in (300, 2000, 2000))
+    q, k, v = (normal(gen, n, 8, 128, dt=F16) for n in (1300, 2000, 2000))
     q1 = q[:2].contiguous()
-    offs = [torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0, 300], [0], [2000], [0, 2])]
-    pos = torch.arange(300, device="cuda", dtype=torch.int32)
+    offs = [torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0, 1300], [0], [2000], [0, 2])]
+    pos = torch.arange(1300, device="cuda", dtype=torch.int32)
     freq, mag = inv_freq(0, 1e6, 128, 1.0, 0.0, 0.0, 0.0)
     err = torch.zeros(1, dtype=torch.int32, device="cuda")
 
@@ -353,8 +355,8 @@ def test_repeats_streams_and_graphs_give_the_same_bits(gen):
         check(L.nemo_op_w4_matvec(E4M3, wx.data_ptr(), 4096, xs.data_ptr(), 128, w4.data_ptr(), F16, s.data_ptr(),
                                   z4.data_ptr(), 64, 3, 1024, 4096, F32, b["y"].data_ptr(), 1024, st))
         check(L.nemo_op_rope_apply(F16, 0, q.data_ptr(), 1024, 8, None, 0, 0, 128, 128, freq.data_ptr(), mag,
-                                   pos.data_ptr(), 300, b["ro"].data_ptr(), 1024, None, 0, st))
-        for qq, off, n, o in ((b["ro"], offs[0], 300, b["at"]), (q1, offs[3], 2, b["a1"])):
+                                   pos.data_ptr(), 1300, b["ro"].data_ptr(), 1024, None, 0, st))
+        for qq, off, n, o in ((b["ro"], offs[0], 1300, b["at"]), (q1, offs[3], 2, b["a1"])):
             check(L.nemo_op_attention_window(F16, qq.data_ptr(), 1024, k.data_ptr(), 1024, v.data_ptr(), 1024, 8, 8,
                                              128, off.data_ptr(), offs[1].data_ptr(), offs[2].data_ptr(), 1, n, 2000,
                                              n, 2000, 700, 0, 4, 0.08, o.data_ptr(), 1024, err.data_ptr(), st))
