@@ -131,7 +131,7 @@ struct alignas(16) Pair {
 // them there instead of waiting for the request's offsets between two pairs.
 struct Items {
   const int* before;   // items of the requests before each one, [requests + 1]
-  const Pair* listed;  // items blockIdx.x + i * gridDim.x
+  const Pair* listed;  // items nth(0), nth(1), ...
   int batch, b;
   __device__ __forceinline__ Items(const int* s, const Pair* p, int n) : before(s), listed(p), batch(n), b(0) {}
   __device__ __forceinline__ int total() const { return before[batch]; }
@@ -143,9 +143,14 @@ struct Items {
     // short pairs level the blocks at the end
     return Pair(a, b, in - pair * a.kv_heads, each - 1 - pair);
   }
-  __device__ __forceinline__ Pair at(const AttnWindowArgs& a, int item) {
-    const int i = (item - blockIdx.x) / gridDim.x;
-    return i < kListed ? listed[i] : find(a, item);
+  // The block's i-th item: every other round of the blocks runs backwards, so
+  // that the blocks with the longest pairs of one round get the shortest of the
+  // next (8192 causal queries: 178 us without, 167).
+  __device__ __forceinline__ int nth(int i) const {
+    return i * (int)gridDim.x + (i & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+  }
+  __device__ __forceinline__ Pair at(const AttnWindowArgs& a, int i) {
+    return i < kListed ? listed[i] : find(a, nth(i));
   }
 };
 
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(384, 1)
   const int total = items.total();
   if (threadIdx.x < kListed) {
     Items mine(before, listed, a.batch);
-    const int item = blockIdx.x + threadIdx.x * gridDim.x;
+    const int item = mine.nth(threadIdx.x);
     if (item < total) listed[threadIdx.x] = mine.find(a, item);
   }
   __syncthreads();
@@ -279,8 +284,8 @@ __global__ void __launch_bounds__(384, 1)
     // ---- copies: the elected lane of the converged warp issues them ----
     int n = 0, issued_q = 0;  // K/V tiles and Q pairs issued
     bool ok = true;
-    for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
-      const Pair p = items.at(a, item);
+    for (int i = 0; items.nth(i) < total && ok; ++i) {
+      const Pair p = items.at(a, i);
       if (!p.tiles) continue;
       ok = __all_sync(0xffffffffu, dev::mbar_wait(q_empty, (issued_q & 1) ^ 1, a.err));
       if (!ok) break;
@@ -334,8 +339,8 @@ __global__ void __launch_bounds__(384, 1)
       uint32_t n = 0, nq = 0;                    // K/V tiles whose S, and Q pairs that, have been reached
       uint32_t s_count = 0, p_count = 0;         // S tiles issued, P tiles used
       bool ok = true;
-      for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
-        const Pair p = items.at(a, item);
+      for (int i = 0; items.nth(i) < total && ok; ++i) {
+        const Pair p = items.at(a, i);
         if (!p.tiles) continue;
         const Unit u = p.unit(t);
         if (!dev::mbar_wait(q_full, nq & 1, a.err)) break;
@@ -405,8 +410,8 @@ __global__ void __launch_bounds__(384, 1)
     // zeros first ----
     uint32_t n = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
-      const Pair p = items.at(a, item);
+    for (int i = 0; items.nth(i) < total && ok; ++i) {
+      const Pair p = items.at(a, i);
       for (int j = 0; j < p.tiles; ++j, ++n) {
         const uint32_t st = n % C::kStages;
         ok = __all_sync(0xffffffffu, dev::mbar_wait(kv_full + 8 * st, n / C::kStages & 1, a.err));
@@ -435,8 +440,8 @@ __global__ void __launch_bounds__(384, 1)
     const float scale = a.scale * 1.4426950408889634f;  // scores in log2 units
     int count = 0;  // tiles of this unit so far, over all pairs
     bool ok = true;
-    for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
-      const Pair p = items.at(a, item);
+    for (int i = 0; items.nth(i) < total && ok; ++i) {
+      const Pair p = items.at(a, i);
       const Unit u = p.unit(t);
       if (!u.rows) continue;
       const int p_warp = u.i0 + quarter * 32 + p.rq.nk - p.rq.nq;
@@ -494,7 +499,7 @@ __global__ void __launch_bounds__(384, 1)
         }
         if (!done) {
           sum = make_float2(0.f, 0.f);
-          float tmax = -INFINITY;
+          float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             if (!(any >> c & 1)) continue;
@@ -505,9 +510,11 @@ __global__ void __launch_bounds__(384, 1)
               for (int i = 0; i < 32; ++i) s[c * 32 + i] = bits >> i & 1 ? s[c * 32 + i] : -INFINITY;
             }
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) tmax = dev::max3(tmax, s[c * 32 + i], s[c * 32 + i + 1]);
+            for (int i = 0; i < 32; i += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) part[k] = dev::max3(part[k], s[c * 32 + i + 2 * k], s[c * 32 + i + 2 * k + 1]);
           }
-          tmax *= scale;
+          const float tmax = scale * fmaxf(dev::max3(part[0], part[1], part[2]), part[3]);
           const bool move = __any_sync(0xffffffffu, tmax > m + (whole == 3 ? 0.f : kMaxSlack));
           const float mnew = move ? fmaxf(m, tmax) : m;
           const float neg = mnew == -INFINITY ? 0.f : -mnew;  // no key seen yet: all weights 0
@@ -606,8 +613,8 @@ __global__ void __launch_bounds__(384, 1)
   // Some row met an infinity or NaN, perhaps one that it does not see (weight 0
   // times the value): rows whose result is not finite are computed again.
   Items again(before, listed, a.batch);
-  for (int item = blockIdx.x; item < total; item += gridDim.x) {
-    const Pair p = again.at(a, item);
+  for (int i = 0; again.nth(i) < total; ++i) {
+    const Pair p = again.at(a, i);
 #pragma unroll 1
     for (int t = 0; t < 2; ++t) {
       const Unit u = p.unit(t);

@@ -220,6 +220,20 @@ def test_attention_window_head_layouts(gen, hq, hk):
         ref.check_attention(*args, 257, 0, 4, got)
 
 
+def test_attention_window_more_requests_than_one_launch_takes(gen):
+    qs = [1 + (37 * i) % 130 for i in range(1100)]
+    args = packed(gen, F16, qs, [n + i % 3 for i, n in enumerate(qs)], 2, 1, 64)
+    got = ref.attention(*args, 40, 3, 2)
+    ref.check_attention(*args, 40, 3, 2, got)
+
+
+def test_attention_window_more_work_than_a_block_lists(gen):
+    """Over 50 pairs of 128-row tiles for each SM."""
+    args = packed(gen, BF16, [1000 + i for i in range(64)], [1000 + i for i in range(64)], 32, 4, 64)
+    got = ref.attention(*args, 100, 20, 1)
+    ref.check_attention(*args, 100, 20, 1, got)
+
+
 def test_attention_window_rows_without_keys_are_zeros(gen):
     args = packed(gen, F16, [200, 5], [40, 0], 4, 2, 64)
     got = ref.attention(*args, -1, 0, 0)
