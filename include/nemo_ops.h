@@ -223,7 +223,8 @@ int nemo_rope_inv_freq(int scaling, double theta, int rotary_dim, double factor,
  * row (as nemo_op_rmsnorm_q8 writes them, where group 0 is x_group >= k);
  * 16-bit x takes NULL. y is F16, BF16 or F32. Products q - zero are exact and
  * sums are f32; y is rounded once. m > 16 is refused: nemo_op_qmatmul serves
- * batches. d_x and ldx need the alignment of one element only. */
+ * batches. n and k are at most 2^30. d_x and ldx need the alignment of one
+ * element only. */
 int nemo_op_w4_matvec(int x_dtype, const void* d_x, int64_t ldx, const void* d_x_scales, int x_group, const void* d_w4,
                       int scale_dtype, const void* d_scales, const void* d_zeros, int group, int m, int n, int k,
                       int y_dtype, void* d_y, int64_t ldy, void* stream);
@@ -238,16 +239,18 @@ int nemo_op_w4_matvec(int x_dtype, const void* d_x, int64_t ldx, const void* d_x
  *   j < key length  and  (right < 0 or j <= p + right)
  *   and  (left < 0 or j >= p - left or j < sinks).
  * right 0 is causal, right < 0 with left < 0 bidirectional. A query that sees
- * no key gets zeros. Scores are q . k * scale with an f32 softmax, weights are
- * rounded to dtype for the product with v, which sums in f32. Infinities and
- * NaN in keys or values that a query does not see do not reach its row.
- * dtype F16 or BF16; head_dim 64 or 128; q_heads a multiple of kv_heads; heads
- * follow one another within a row; buffers 16-byte aligned, leading dimensions
- * multiples of 8. q_rows, k_rows: rows of the buffers. max_q: the longest
- * query length (rows past it are not written). max_k: about the longest key
- * length, which only steers the split of the work. Rows of d_out that no
- * request covers stay as they are. d_err is a zeroed 4-byte device word that
- * becomes nonzero if a bounded wait gave up. */
+ * no key, or whose scores are all -infinity, gets zeros. Scores are q . k *
+ * scale with an f32 softmax, weights are rounded to dtype for the product with
+ * v, which sums in f32. Infinities and NaN in keys or values that a query does
+ * not see do not reach its row. dtype F16 or BF16; head_dim 64 or 128; q_heads
+ * a multiple of kv_heads; heads follow one another within a row; batch and
+ * heads at most 65535; buffers 16-byte aligned, leading dimensions multiples
+ * of 8. q_rows, k_rows: rows of the buffers, in which the offsets have to lie.
+ * Requests may share keys. max_q: the longest query length (rows past it are
+ * not written). max_k: about the longest key length, which only steers the
+ * split of the work. Rows of d_out that no request covers stay as they are.
+ * d_err is a zeroed 4-byte device word that becomes nonzero if a bounded wait
+ * gave up. */
 int nemo_op_attention_window(int dtype, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v,
                              int64_t ldv, int q_heads, int kv_heads, int head_dim, const void* d_q_off,
                              const void* d_k_start, const void* d_k_len, int batch, int q_rows, int k_rows, int max_q,

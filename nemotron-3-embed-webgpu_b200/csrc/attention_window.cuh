@@ -63,7 +63,8 @@ struct KeyRange {
 // warp, key by key and touching only keys that the query sees. The tiled
 // kernels multiply weights of 0 with values of keys that other queries of the
 // tile see; where such a value is infinite or NaN the product is NaN, and the
-// rows it reached are computed again here.
+// rows it reached are computed again here (up to the key that settles the row,
+// so that a call on NaN throughout does not crawl).
 template <typename T>
 __device__ __noinline__ void attention_row(const AttnWindowArgs& a, AttnRequest r, int i, int head, int d0,
                                            int d1) {
@@ -83,14 +84,22 @@ __device__ __noinline__ void attention_row(const AttnWindowArgs& a, AttnRequest 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     s *= a.scale * 1.4426950408889634f;
-    // a NaN or +infinity score makes the row NaN, as it does in a softmax
+    if (!(s < INFINITY)) {  // a NaN or +infinity score makes the row NaN, as it does in a softmax
+      l = __uint_as_float(0x7fc00000u);
+      break;
+    }
     const float mn = fmaxf(m, s);
     const float keep = m == -INFINITY ? 0.f : exp2f(m - mn);
     const float w = s == -INFINITY ? 0.f : exp2f(s - mn);
     l = l * keep + w;
+    bool lost = true;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (c * 32 + lane < d) acc[c] = acc[c] * keep + w * dev::to_f32(v[(int64_t)j * a.ldv + c * 32 + lane]);
+      if (c * 32 + lane < d) {
+        acc[c] = acc[c] * keep + w * dev::to_f32(v[(int64_t)j * a.ldv + c * 32 + lane]);
+        lost &= isnan(acc[c]);
+      }
+    if (__all_sync(0xffffffffu, lost)) break;  // every column is NaN: no later key changes that
     m = mn;
   }
   T* out = static_cast<T*>(a.out) + (int64_t)(r.q0 + i) * a.ldo + head * d;

@@ -6,10 +6,13 @@
 // group) pairs of one kv head, which is what an m16n8k16 instruction takes; a
 // 128-row tcgen05 tile would be nearly empty. The keys are split over the 4
 // warps of a block and over the blocks of a cluster, each warp running its own
-// online softmax over chunks of 32 keys that it copies to shared memory
+// online softmax over chunks of 16 keys that it copies to shared memory
 // itself (no block barriers in the loop); the partial results meet in shared
-// memory and, over the cluster, in distributed shared memory, always in the
-// same order.
+// memory and, over the cluster, in the shared memory of the block that writes
+// their columns, always in the same order. 16 tokens on up to 5000 keys, window
+// of 1024 and four sinks, 24 + 8 heads of 128 (f16): 16.4 us, 4.1 TB/s of the
+// visible rows. A warp has only two or three chunks there, so the first copies
+// and the two merges, not the stream between them, are what is left.
 //
 // Scores and statistics are f32; weights are rounded to the 16-bit type for
 // the product with V (relative error half a step, like the output's own

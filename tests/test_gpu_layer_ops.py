@@ -2,6 +2,10 @@
 wrong: sizes around the tiles, strides, groups, windows that leave a row empty, garbage where nothing may look, streams
 and graphs, and one layer's run of them together."""
 import ctypes
+import os
+import subprocess
+import sys
+import threading
 
 import numpy as np
 import pytest
@@ -154,6 +158,16 @@ def test_w4_matvec(gen, xt, group, x_group, m, n, k):
     x, xs, q, s, z = w4_inputs(gen, xt, m, n, k, group, zeros, st, x_group)
     y = ref.w4_matvec(x, xs, x_group, ref.pack4(q), s, ref.pack4(z) if zeros else None, group, n, yt)
     ref.check_w4(x, xs, x_group, q, s, z, group, y, yt)
+
+
+@pytest.mark.parametrize("xt,group,x_group,m,n,k", [
+    (F16, 128, 0, 16, 50, 20480), (E4M3, 32, 64, 12, 9000, 14336), (BF16, 64, 0, 1, 40, 262144),
+    (I8, 128, 32, 3, 2000, 65536), (F16, 32, 0, 16, 3, 12320)])
+def test_w4_matvec_rows_longer_than_a_cluster_holds(gen, xt, group, x_group, m, n, k):
+    """x of a row fills more panels of shared memory than a cluster has blocks: each block takes several in turn."""
+    x, xs, q, s, z = w4_inputs(gen, xt, m, n, k, group, True, F16, x_group or k)
+    y = ref.w4_matvec(x, xs, x_group, ref.pack4(q), s, ref.pack4(z), group, n, F32)
+    ref.check_w4(x, xs, x_group, q, s, z, group, y, F32)
 
 
 def test_w4_matvec_strides_and_odd_addresses(gen):
@@ -311,6 +325,35 @@ def test_attention_window_bad_keys_in_the_open(gen, dt, q_len, bad):
         ref.check_attention(*one, -1, -1, 0, got[:, 64:])
 
 
+@TYPES
+@pytest.mark.parametrize("q_len,hq", [(1, 2), (200, 2), (1200, 8)])
+def test_attention_window_nothing_but_bad_values(gen, dt, q_len, hq):
+    """Keys of NaN make every row NaN, values of NaN too; scores that are all -infinity count for nothing."""
+    args = packed(gen, dt, [q_len], [1200], hq, 1, 64)
+    q, k, v = args[:3]
+    q.abs_().add_(0.5)
+    for keys, values in ((float("nan"), None), (None, float("nan")), (-float("inf"), None)):
+        kk = k if keys is None else torch.full_like(k, keys)
+        vv = v if values is None else torch.full_like(v, values)
+        got = ref.attention(q, kk, vv, *args[3:], 300, 0, 2)
+        assert (got == 0).all() if keys == -float("inf") else torch.isnan(got).all()
+
+
+@pytest.mark.parametrize("longest", [40, 900])
+def test_attention_window_lengths_that_steer(gen, longest):
+    """max_k changes no result beyond the weights' roundings; rows past max_q are not written; requests share keys."""
+    args = packed(gen, F16, [longest, 3, longest - 7], [1000, 0, 0], 4, 2, 64)
+    args = (*args[:4], [0, 0, 100], [1000, 1000, 900])
+    for max_k in (0, 1, 10 ** 9):
+        got = ref.attention(*args, 200, 0, 4, max_k=max_k)
+        ref.check_attention(*args, 200, 0, 4, got)
+    cut = ref.attention(*args, 200, 0, 4, max_q=30)
+    for b, (q0, q1) in enumerate(zip(args[3], args[3][1:])):
+        n = min(30, q1 - q0)
+        assert (cut[q0 + n:q1] == 7.0).all()
+        ref.close(cut[q0:q0 + n], got[q0:q0 + n].double(), 4 * ref.HALF[F16] * args[2].abs().max().double())
+
+
 @pytest.mark.parametrize("q_len,hq", [(1, 2), (200, 2), (900, 8)])
 def test_attention_window_large_scores(gen, q_len, hq):
     """Scores of several thousand: the largest key takes all the weight, nothing overflows."""
@@ -399,6 +442,79 @@ def test_repeats_streams_and_graphs_give_the_same_bits(gen):
         for name in want:
             assert torch.equal(got[name], want[name]), name
     assert int(err) == 0
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are captured, which is when the kernels are loaded and given their shared memory."""
+    program = """
+import torch, layer_ops_ref as ref
+from nemo_b200.runtime import check, load_library
+L = load_library()
+f = lambda *n: torch.ones(n, dtype=torch.float16, device="cuda")
+x, w, y, o = f(2, 256), torch.ones(256, device="cuda"), f(2, 256), f(700, 256)
+q8, sc = torch.zeros((2, 256), dtype=torch.int8, device="cuda"), torch.zeros((2, 2), device="cuda")
+w4, s = torch.full((256, 128), 0x99, dtype=torch.uint8, device="cuda"), f(256, 2)
+kv, off, i = f(700, 256), [torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0, 2], [0, 700])], 0
+pos, freq = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.ones(32, dtype=torch.float64, device="cuda")
+start, n = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full((1,), 700, dtype=torch.int32, device="cuda")
+err = torch.zeros(1, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    st = ref.stream()
+    check(L.nemo_op_rmsnorm_q8(0, x.data_ptr(), 256, None, 0, w.data_ptr(), 2, 256, 0.0, None, 0, 4, 128, q8.data_ptr(),
+                               256, sc.data_ptr(), st))
+    check(L.nemo_op_w4_matvec(4, q8.data_ptr(), 256, sc.data_ptr(), 128, w4.data_ptr(), 0, s.data_ptr(), None, 128, 2,
+                              256, 256, 0, y.data_ptr(), 256, st))
+    check(L.nemo_op_rope_apply(0, 0, y.data_ptr(), 256, 4, None, 0, 0, 64, 64, freq.data_ptr(), 1.0, pos.data_ptr(), 2,
+                               y.data_ptr(), 256, None, 0, st))
+    for qq, rows, qo in ((y, 2, off[0]), (kv, 700, off[1])):
+        check(L.nemo_op_attention_window(0, qq.data_ptr(), 256, kv.data_ptr(), 256, kv.data_ptr(), 256, 4, 4, 64,
+                                         qo.data_ptr(), start.data_ptr(), n.data_ptr(), 1, rows, 700, rows, 700, -1, 0,
+                                         0, 0.125, o.data_ptr(), 256, err.data_ptr(), st))
+g.replay()
+torch.cuda.synchronize()
+assert (q8 == 127).all() and int(err) == 0 and (o == 1).all()
+# 256 columns of 127 * (1 / 127) * (9 - 8)
+assert ((y.float() - 256).abs() <= 256 * 2.0 ** -11).all()
+print("captured")
+"""
+    run = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300,
+                         env={**os.environ, "PYTHONPATH": ":".join(p for p in sys.path if p)})
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
+
+
+def test_two_host_threads_at_once(gen):
+    """Calls from two threads on their own streams, refused ones among them: each gets its results and its message."""
+    args = packed(gen, F16, [5, 300], [400, 300], 4, 2, 64)
+    x, w = normal(gen, 40, 1000, dt=F16), normal(gen, 1000)
+    want = ref.attention(*args, 50, 0, 1), ref.rmsnorm_q8(x, None, w, 1e-5, I8, 128)[1]
+    wrong = []
+
+    def work(first):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(20):
+                    if (i + first) % 2:
+                        if not torch.equal(ref.attention(*args, 50, 0, 1), want[0]):
+                            wrong.append("attention")
+                        with pytest.raises(NemoError, match="head_dim"):
+                            ref.attention(*[t[..., :32] for t in args[:3]], *args[3:], 50, 0, 1)
+                    else:
+                        if not torch.equal(ref.rmsnorm_q8(x, None, w, 1e-5, I8, 128)[1], want[1]):
+                            wrong.append("norm")
+                        with pytest.raises(NemoError, match="group"):
+                            ref.rmsnorm_q8(x, None, w, 1e-5, I8, 48)
+        except BaseException as e:  # a failed check of this thread
+            wrong.append(repr(e))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_host_memory_is_refused(gen):
