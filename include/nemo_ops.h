@@ -221,8 +221,10 @@ int nemo_rope_inv_freq(int scaling, double theta, int rotary_dim, double factor,
  * divides k. x is F16, BF16, E4M3 or I8; 8-bit codes take d_x_scales f32
  * [m x ceil(k / x_group)], x_group 32, 64 or 128, or >= k for one scale per
  * row (as nemo_op_rmsnorm_q8 writes them, where group 0 is x_group >= k);
- * 16-bit x takes NULL. y is F16, BF16 or F32. Products q - zero are exact and
- * sums are f32; y is rounded once. m > 16 is refused: nemo_op_qmatmul serves
+ * 16-bit x takes NULL. y is F16, BF16 or F32. Sums are f32 or finer and y is
+ * rounded once; 16-bit elements of x below 2^-19 of the largest of their 32 to
+ * 128 neighbours may be rounded to 2^-30 of it. An infinity or NaN in a row of
+ * x makes its row of y infinite or NaN. m > 16 is refused: nemo_op_qmatmul serves
  * batches. n and k are at most 2^30. d_x and ldx need the alignment of one
  * element only. */
 int nemo_op_w4_matvec(int x_dtype, const void* d_x, int64_t ldx, const void* d_x_scales, int x_group, const void* d_w4,

@@ -3,20 +3,29 @@
 //
 //   y[m][r] = sum_g s[r][g] * ( sum_{c in g} x[m][c] * (q[r][c] - z[r][g]) )
 //
-// The inner sum runs on m16n8k16 tensor-core instructions: A = 16 weight rows
-// as the exact small integers q - z in the type of x, B = up to 8 rows of x,
-// f32 accumulation; each segment's sum is then scaled in f32. Nothing is
-// rounded before y. (The 128-row tcgen05 tile would hold 16 rows of x against
-// 128 of weights, but its operand would have to be written to shared or tensor
-// memory; here the decoded integers go from registers straight into the
-// instruction, and the bound is the stream of weights, not the tensor rate.)
+// The inner sum runs on tensor-core instructions whose A is 16 weight rows and
+// whose B holds up to 8 columns made from x; each segment's sum is then scaled in
+// f32. (The 128-row tcgen05 tile would hold 16 rows of x against 128 of weights,
+// but its operand would have to be written to shared or tensor memory; here the
+// decoded integers go from registers straight into the instruction, and the
+// bound is the stream of weights, not the tensor rate.) Two forms:
+//
+//   floating point (m16n8k16): A = the exact small integers q - z in the type of
+//   x, B = up to 8 rows of x, f32 accumulation. A word of 8 nibbles takes 9
+//   instructions to decode in f16, 11 in bf16.
+//
+//   digits (m16n8k32, integers): A = the nibbles q themselves, two masks and a
+//   shift a word, B = the 8-bit digits of x as fixed-point numbers, four columns
+//   a row of x (load_digits; i8 codes are one column). The sums are whole
+//   numbers without any rounding; -z * (sum of the digits) is where they start.
 //
 // A segment is the shorter of the weight group and the group of x scales (32,
 // 64 or 128 columns). A lane takes SEG/32 consecutive 32-bit words of a row per
 // segment: the columns that an instruction's k index stands for are permuted,
 // in the same way for the weights and for x, so that each lane reads its
-// weights as one vector and each word's nibble pairs (k, k + 4) come out of
-// one mask; x is stored in shared memory in that order.
+// weights as one vector and the nibbles of a word that belong together come out
+// of one mask (pairs (k, k + 4), or the even and the odd ones); x is stored in
+// shared memory in that order.
 //
 // A warp's work is 16 R rows and a slice of a panel of columns, in chunks of 256
 // columns (R x 2 KB). Each warp copies its own next chunks and their scales to
@@ -25,14 +34,19 @@
 // where there are rows enough for every warp of the GPU, so that nothing is
 // summed over warps; more where there are few rows. Panels (of the columns
 // whose x fits shared memory) of a row tile are blocks of one cluster, summed in
-// rank order through distributed shared memory.
+// rank order through distributed shared memory. (Chunks of all the block's tiles
+// in one stream, an eighth for each warp, balance better, 28.9 us where this
+// took 31.0, but the sums of tiles that warps share cost 0.3 us in small calls and
+// twice the time where a row takes several panels.)
 //
 // Bound: at 6.5 TB/s an SM gets 4 KB of weights (32 rows x 256 columns) in 180
-// cycles, in which its schedulers issue 720 instructions; decoding and
-// multiplying them takes some 450 and the chunk's copies and scales 300. One row
-// of bf16 x against 131072 x 2048: 40 us, 3.5 TB/s (16-row tiles 61, a fixed
-// split of every tile over the 8 warps 51, 64 with the scales read in line and
-// two logic operations a nibble pair); one row against 5120 x 2048: 5.2 us.
+// cycles, in which its schedulers issue 720 instructions; the floating-point form
+// takes some 750 for them, digits about 450. One row of bf16 x against 131072 x
+// 2048: 29.0 us with digits, 4.8 TB/s (37.7 without); 512 tiles are 1.7 rounds of
+// 296 blocks, and the last round is the most of what is missing. (16-row tiles
+// 61, a fixed split of every tile over the 8 warps 51, 64 with the scales read in
+// line and two logic operations a nibble pair, all without digits.) One row
+// against 5120 x 2048: 4.9 us.
 #include <type_traits>
 
 #include "layer_ops.cuh"
@@ -58,7 +72,7 @@ struct W4Plan {
   int tiles;       // block tiles (8 / wk x 16 R rows)
   int blocks;      // blocks over the tiles
   int stages;      // chunks in flight
-  int mp;          // rows of x in shared memory: m rounded up to 1, 2, 4, 8 or 16
+  int cols;        // columns of x's operand in shared memory: m rounded up to 1, 2, 4, 8 or 16, or m's digits
   int off_x, off_xs, off_zero, off_red;  // byte offsets in shared memory (the warps' stages at 0)
 };
 
@@ -119,6 +133,17 @@ struct Nibbles<__nv_bfloat16> {
   }
 };
 
+// D[16 x 8] += A[16 x 32] . B[32 x 8], unsigned by signed 8-bit integers, in one warp.
+__device__ __forceinline__ void mma_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+constexpr int kMagic = 0x4b400000;  // 1.5 * 2^23 as bits: plus i, |i| < 2^22, the bits of 1.5 * 2^23 + i
+
 // Eight elements of x as they lie in memory: 16 bytes of 16-bit ones, 8 of codes.
 template <bool CODES>
 __device__ __forceinline__ uint4 load_x8(const void* x, int64_t at) {
@@ -143,23 +168,24 @@ __device__ __forceinline__ uint4 load_x8(const void* x, int64_t at) {
     return make_uint4(v[0], v[1], v[2], v[3]);
   }
 }
-// The same in the type of the products (codes without their scale, exact in
-// f16), paired as one word's nibbles are: (0, 4), (1, 5), (2, 6), (3, 7).
-template <bool CODES>
-__device__ __forceinline__ uint4 pair_x8(uint4 u, int dtype) {
-  uint32_t v[4] = {u.x, u.y, u.z, u.w};
-  if constexpr (CODES) {
+// Codes as f16 (exact).
+__device__ __forceinline__ uint4 codes_to_f16(uint4 u, int dtype) {
+  uint32_t v[4];
 #pragma unroll
-    for (int i = 3; i >= 0; --i) {
-      const uint32_t two = v[i / 2] >> (i & 1) * 16;
-      if (dtype == kDtE4M3) {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffff), __NV_E4M3);
-        v[i] = h.x | (uint32_t)h.y << 16;
-      } else {
-        v[i] = dev::pack2<__half>((float)(int8_t)(two & 0xff), (float)(int8_t)(two >> 8 & 0xff));
-      }
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t two = (i < 2 ? u.x : u.y) >> (i & 1) * 16;
+    if (dtype == kDtE4M3) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffff), __NV_E4M3);
+      v[i] = h.x | (uint32_t)h.y << 16;
+    } else {
+      v[i] = dev::pack2<__half>((float)(int8_t)(two & 0xff), (float)(int8_t)(two >> 8 & 0xff));
     }
   }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+// Eight 16-bit elements paired as one word's nibbles are: (0, 4), (1, 5), (2, 6), (3, 7).
+__device__ __forceinline__ uint4 pair_x8(uint4 u) {
+  const uint32_t v[4] = {u.x, u.y, u.z, u.w};
   return make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), __byte_perm(v[1], v[3], 0x5410),
                     __byte_perm(v[1], v[3], 0x7632));
 }
@@ -177,16 +203,18 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// T: type of the products (f16 also for 8-bit x, whose codes it holds
-// exactly). R: 16-row tiles per block. NT: 8-row tiles of x. XG: x scales per
-// group.
+// T: type of the products (f16 also for 8-bit x, which it holds exactly; int8_t:
+// digits). R: 16-row tiles per warp. NT: 8-column tiles of x's operand. XG: x
+// scales per group (always with digits).
 template <typename T, int SEG, int R, int NT, bool XG>
 __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_constant__ W4Plan p) {
   extern __shared__ __align__(128) uint8_t smem[];
   using C = W4Cfg<SEG, R>;
   constexpr int WPL = SEG / 32;  // words of a row per lane and segment
-  constexpr int ROWS = C::kRows, COLS = 8 * NT;
+  constexpr int ROWS = C::kRows;
   constexpr int SEG_BYTES = SEG / 2, CHUNK_SEGS = kChunk / SEG;
+  constexpr bool DIGITS = std::is_same<T, int8_t>::value;
+  constexpr int XW = DIGITS ? (WPL < 2 ? 1 : 2) : 1;  // words of a lane whose x is one read of 16 (8 with WPL 1) bytes
   const W4Args& a = p.a;
   dev::pdl_launch_dependents();
   dev::pdl_wait();
@@ -196,8 +224,9 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
   const int block_rows = row_tiles * ROWS;
   uint8_t* stages = smem + warp * p.stages * C::kStage;
   uint8_t* sx = smem + p.off_x;
-  float* sxs = reinterpret_cast<float*>(smem + p.off_xs);
-  float* red = reinterpret_cast<float*>(smem + p.off_red);  // two buffers of [wk][COLS][block_rows]
+  float* sxs = reinterpret_cast<float*>(smem + p.off_xs);            // [segment][column]
+  int* sums = reinterpret_cast<int*>(sxs + p.panel_segs * p.cols);   // of the digits, alike
+  float* red = reinterpret_cast<float*>(smem + p.off_red);  // two buffers of [wk][row of x][block_rows]
   const int groups = a.k / a.group;
   const int seg_shift = a.group == SEG ? 0 : a.group == 2 * SEG ? 1 : 2;  // segments of a group, log2
   const int zero_bytes = (groups + 1) / 2;
@@ -252,15 +281,17 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
   auto load = [&](int stage) {
     if (next.tile < p.tiles && unit < next.left * (SEG_BYTES / 16)) {
       const uint32_t to = dev::smem_u32(stages) + stage * C::kStage + r0 * kPitch;
-      const uint8_t* from = w_from;
+      if (whole) {
+        const uint8_t* from = w_from;
 #pragma unroll
-      for (int i = 0; i < ROWS / 4; ++i) {
-        if (!whole) {
-          const int row0 = next.tile * block_rows + wr * ROWS;
-          from = w_from + (int64_t)(min(row0 + i * 4 + r0, a.n - 1) - row0 - r0) * row_bytes;
-        }
-        dev::cp_async16(to + i * 4 * kPitch + (unit ^ ((i * 4 + r0) % (8 / WPL) * WPL)) * 16, from);
-        from += 4 * row_bytes;
+        for (int i = 0; i < ROWS / 4; ++i, from += 4 * row_bytes)
+          dev::cp_async16(to + i * 4 * kPitch + (unit ^ ((i * 4 + r0) % (8 / WPL) * WPL)) * 16, from);
+      } else {
+        const int row0 = next.tile * block_rows + wr * ROWS;
+#pragma unroll 1
+        for (int i = 0; i < ROWS / 4; ++i)
+          dev::cp_async16(to + i * 4 * kPitch + (unit ^ ((i * 4 + r0) % (8 / WPL) * WPL)) * 16,
+                          w_from + (int64_t)(min(row0 + i * 4 + r0, a.n - 1) - row0 - r0) * row_bytes);
       }
     }
     dev::cp_async_commit();
@@ -292,8 +323,9 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
       const uint16_t bits = (uint16_t)scale16[j];
       const float f = a.scale_dtype == kDtBF16 ? __uint_as_float(scale16[j] << 16)
                                                : __half2float(*reinterpret_cast<const __half*>(&bits));
-      if (i < C::kGroups)
-        ss[i * ROWS + own_row] = make_uint2(__float_as_uint(f), (Nibbles<T>::kBase + (zero4[j] & 15)) * 0x10001u);
+      uint32_t zero = zero4[j] & 15;
+      if constexpr (!DIGITS) zero = (Nibbles<T>::kBase + zero) * 0x10001u;
+      if (i < C::kGroups) ss[i * ROWS + own_row] = make_uint2(__float_as_uint(f), zero);
     }
   };
   // x of a panel in the order of the instructions: for each 32-column step of a
@@ -303,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
     const int seg0 = panel * p.panel_segs, n = min(p.panel_segs, p.segs - seg0);
     const int units = n * (SEG / 8);  // of a row
     constexpr int kAhead = 4;         // loads in flight
-    for (int i0 = threadIdx.x; i0 < p.mp * units; i0 += kAhead * kThreads) {
+    for (int i0 = threadIdx.x; i0 < p.cols * units; i0 += kAhead * kThreads) {
       uint4 raw[kAhead];
       int to[kAhead];
 #pragma unroll
@@ -311,25 +343,123 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
         const int i = i0 + j * kThreads;
         const int m = i / units, u = i - m * units;
         const int seg = u / (SEG / 8), rem = u % (SEG / 8);
-        to[j] = i < p.mp * units ? (((seg * WPL + rem % WPL) * p.mp + m) * 4 + rem / WPL) * 16 : -1;
+        to[j] = i < p.cols * units ? (((seg * WPL + rem % WPL) * p.cols + m) * 4 + rem / WPL) * 16 : -1;
         raw[j] = make_uint4(0, 0, 0, 0);
-        if (m < a.m && i < p.mp * units) raw[j] = load_x8<CODES>(a.x, m * a.ldx + (int64_t)seg0 * SEG + u * 8);
+        if (m < a.m && i < p.cols * units) raw[j] = load_x8<CODES>(a.x, m * a.ldx + (int64_t)seg0 * SEG + u * 8);
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j)
-        if (to[j] >= 0) *reinterpret_cast<uint4*>(sx + to[j]) = pair_x8<CODES>(raw[j], a.x_dtype);
+        if (to[j] >= 0) *reinterpret_cast<uint4*>(sx + to[j]) = pair_x8(CODES ? codes_to_f16(raw[j], a.x_dtype) : raw[j]);
     }
     if (XG)
-      for (int i = threadIdx.x; i < n * p.mp; i += kThreads) {
-        const int m = i % p.mp, seg = i / p.mp;
+      for (int i = threadIdx.x; i < n * p.cols; i += kThreads) {
+        const int m = i % p.cols, seg = i / p.cols;
         sxs[i] = m < a.m ? a.x_scales[(int64_t)m * x_groups + (int64_t)(seg0 + seg) * SEG / a.x_group] : 0.f;
       }
   };
-  auto stage_x = [&](int panel) {
-    if (a.x_dtype == kDtE4M3 || a.x_dtype == kDtI8) load_x(panel, std::true_type{});
-    else load_x(panel, std::false_type{});
+  // The same as digits: element x of a segment whose largest magnitude is below
+  // 2^(e + 1) is the integer X = x 2^(29 - e), |X| <= 2^30 (exact where x is at
+  // least 2^-19 of the largest, otherwise rounded to 2^-30 of it), in four
+  // balanced digits of 8 bits, a column of the operand each (column 4 m + s:
+  // digit s, worth 2^(8 s + e - 29)). i8 codes are a digit themselves. Eight
+  // elements a thread, the segment's lanes side by side.
+  auto load_digits = [&](int panel, auto kind) {
+    constexpr int KIND = decltype(kind)::value;  // dtype of x
+    constexpr bool CODES = KIND == kDtE4M3 || KIND == kDtI8;
+    constexpr int LANES = SEG / 8;
+    const int seg0 = panel * p.panel_segs, n = min(p.panel_segs, p.segs - seg0);
+    const int units = n * LANES, rows = KIND == kDtI8 ? p.cols : a.m;
+    constexpr int kAhead = 4;
+    for (int m = 0; m < rows; ++m)
+    for (int u0 = threadIdx.x - lane; u0 < units; u0 += kAhead * kThreads) {  // (of the warp)
+      uint4 raw[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int u = u0 + j * kThreads + lane;
+        raw[j] = make_uint4(0, 0, 0, 0);
+        if (u < units && m < a.m) raw[j] = load_x8<CODES>(a.x, m * a.ldx + (int64_t)seg0 * SEG + u * 8);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (u0 + j * kThreads >= units) break;
+        const int u = u0 + j * kThreads + lane;
+        const int seg = u / LANES, rem = u % LANES, word = rem % WPL;
+        const bool in = u < units;
+        float xs = 1.f;
+        if (in && a.x_group < a.k)
+          xs = m < a.m ? a.x_scales[(int64_t)m * x_groups + (int64_t)(seg0 + seg) * SEG / a.x_group] : 0.f;
+        const int at = (seg * (WPL / XW) + word / XW) * p.cols;  // the columns' rows of 4 lanes
+        uint8_t* to = sx + (rem / WPL) * (XW * 8) + word % XW * 8;
+        if constexpr (KIND == kDtI8) {
+          const uint32_t even = __byte_perm(raw[j].x, raw[j].y, 0x6420), odd = __byte_perm(raw[j].x, raw[j].y, 0x7531);
+          int sum = __dp4a((int)even, 0x01010101, __dp4a((int)odd, 0x01010101, 0));
+#pragma unroll
+          for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (in) {
+            *reinterpret_cast<uint2*>(to + (at + m) * (XW * 32)) = make_uint2(even, odd);
+            if (rem == 0) sxs[seg * p.cols + m] = xs, sums[seg * p.cols + m] = sum;
+          }
+        } else {
+          float v[8];
+          if constexpr (KIND == kDtBF16) dev::unpack8<__nv_bfloat16>(raw[j], v);
+          else dev::unpack8<__half>(KIND == kDtE4M3 ? codes_to_f16(raw[j], KIND) : raw[j], v);
+          uint32_t top = 0;  // as integers magnitudes compare like floats, NaN above infinity
+#pragma unroll
+          for (int c = 0; c < 8; ++c) top = max(top, __float_as_uint(v[c]) & 0x7fffffffu);
+#pragma unroll
+          for (int o = 1; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int e = max((int)(top >> 23) - 127, -97);  // 2^(29 - e) and its inverse are normal
+          const float up = __uint_as_float((uint32_t)(156 - e) << 23);
+          uint32_t d[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) d[c] = ((uint32_t)__float2int_rn(v[c] * up) + 0x00808080u) ^ 0x00808080u;
+          uint32_t half[2][4];  // of even and odd columns, the digits s of four elements
+          int sum[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t a01 = __byte_perm(d[h], d[2 + h], 0x5140), a23 = __byte_perm(d[4 + h], d[6 + h], 0x5140);
+            const uint32_t b01 = __byte_perm(d[h], d[2 + h], 0x7362), b23 = __byte_perm(d[4 + h], d[6 + h], 0x7362);
+            half[h][0] = __byte_perm(a01, a23, 0x5410), half[h][1] = __byte_perm(a01, a23, 0x7632);
+            half[h][2] = __byte_perm(b01, b23, 0x5410), half[h][3] = __byte_perm(b01, b23, 0x7632);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            sum[c] = __dp4a((int)half[0][c], 0x01010101, __dp4a((int)half[1][c], 0x01010101, 0));
+          // two sums of at most 2^14 in a word
+          int low = sum[0] + sum[1] * 65536, high = sum[2] + sum[3] * 65536;
+#pragma unroll
+          for (int o = 1; o < LANES; o <<= 1) {
+            low += __shfl_xor_sync(0xffffffffu, low, o);
+            high += __shfl_xor_sync(0xffffffffu, high, o);
+          }
+          if (in) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              *reinterpret_cast<uint2*>(to + (at + 4 * m + c) * (XW * 32)) = make_uint2(half[0][c], half[1][c]);
+            if (rem < 4) {  // a lane of the segment for each digit
+              const int pair = rem & 2 ? high : low, first = (int16_t)(pair & 0xffff);
+              sums[seg * p.cols + 4 * m + rem] = rem & 1 ? (pair - first) >> 16 : first;
+              // an infinity or NaN makes every product of the row NaN
+              sxs[seg * p.cols + 4 * m + rem] =
+                  top < 0x7f800000u ? xs * __uint_as_float((uint32_t)(e + 98 + 8 * rem) << 23) : __uint_as_float(0x7fc00000u);
+            }
+          }
+        }
+      }
+    }
   };
-
+  auto stage_x = [&](int panel) {
+    if constexpr (DIGITS) {
+      if (a.x_dtype == kDtF16) load_digits(panel, std::integral_constant<int, kDtF16>{});
+      else if (a.x_dtype == kDtBF16) load_digits(panel, std::integral_constant<int, kDtBF16>{});
+      else if (a.x_dtype == kDtE4M3) load_digits(panel, std::integral_constant<int, kDtE4M3>{});
+      else load_digits(panel, std::integral_constant<int, kDtI8>{});
+    } else if (a.x_dtype == kDtE4M3 || a.x_dtype == kDtI8) {
+      load_x(panel, std::true_type{});
+    } else {
+      load_x(panel, std::false_type{});
+    }
+  };
 
   const int ahead = p.stages - 1;
   aim();
@@ -349,14 +479,15 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
     stage_x(rank);
     __syncthreads();
   }
-  // the lane's rows of x; those past the last one read zeros behind it
+  // the lane's columns of the operand; those past the last one read zeros behind it
+  constexpr int XB = DIGITS ? XW * 8 : 16;  // bytes of a read
   const uint8_t* x_at[NT];
   int x_step[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const bool live = n * 8 + g < p.mp;
-    x_at[n] = live ? sx + ((n * 8 + g) * 4 + t) * 16 : smem + p.off_zero;
-    x_step[n] = live ? p.mp * 64 : 0;
+    const bool live = n * 8 + g < p.cols;
+    x_at[n] = live ? sx + ((n * 8 + g) * 4 + t) * XB : smem + p.off_zero;
+    x_step[n] = live ? p.cols * 4 * XB : 0;
   }
   float acc[R][NT][4];
 #pragma unroll
@@ -385,12 +516,12 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
     const int flip = g % (8 / WPL) * WPL * 16;
     const uint8_t* xp[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) xp[n] = x_at[n] + in_panel * WPL * x_step[n];
+    for (int n = 0; n < NT; ++n) xp[n] = x_at[n] + in_panel * (WPL / XW) * x_step[n];
 #pragma unroll
     for (int s = 0; s < CHUNK_SEGS; ++s) {
       if (s >= n_segs) break;
       const uint2* sp = ss + (((seg0 + s) >> seg_shift) - g0) * ROWS + g;
-      uint32_t w[R][2][WPL], zc[R][2], zh[R][2];
+      uint32_t w[R][2][WPL], zc[R][2];
       float sc[R][2];
 #pragma unroll
       for (int r = 0; r < R; ++r)
@@ -400,44 +531,97 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
           const uint2 v = sp[r * 16 + h * 8];
           sc[r][h] = __uint_as_float(v.x);
           zc[r][h] = v.y;
-          zh[r][h] = Nibbles<T>::high(v.y);
         }
-      float part[R][NT][4];
-#pragma unroll
-      for (int j = 0; j < WPL; ++j) {
-        uint4 b[NT];
+      if constexpr (DIGITS) {
+        // whole numbers throughout: the sums start at -zero * (sum of the digits),
+        // and read as f32 they are 1.5 * 2^23 more than themselves
+        float f[NT][2];
+        int part[R][NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          b[n] = *reinterpret_cast<const uint4*>(xp[n]);
-          xp[n] += x_step[n];
+          const int col = n * 8 + 2 * t;
+          float2 fs = make_float2(0.f, 0.f);
+          int2 sd = make_int2(0, 0);
+          if (col < p.cols) {
+            fs = *reinterpret_cast<const float2*>(sxs + (in_panel + s) * p.cols + col);
+            sd = *reinterpret_cast<const int2*>(sums + (in_panel + s) * p.cols + col);
+          }
+          f[n][0] = fs.x, f[n][1] = fs.y;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[r][n][i] = kMagic - (int)zc[r][i >> 1] * (i & 1 ? sd.y : sd.x);
         }
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          uint32_t lo[4], hi[4];
-          Nibbles<T>::decode(w[r][0][j], zc[r][0], zh[r][0], lo);
-          Nibbles<T>::decode(w[r][1][j], zc[r][1], zh[r][1], hi);
+        for (int j = 0; j < WPL; j += XW) {
+          uint32_t b[NT][2 * XW];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            if (j == 0) dev::mma_16816_zero<T>(part[r][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
-            else dev::mma_16816<T>(part[r][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
-            dev::mma_16816<T>(part[r][n], lo[2], hi[2], lo[3], hi[3], b[n].z, b[n].w);
+            lds_words<2 * XW>(xp[n], b[n]);
+            xp[n] += x_step[n];
+          }
+#pragma unroll
+          for (int i = 0; i < XW; ++i)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              const uint32_t w0 = w[r][0][j + i], w1 = w[r][1][j + i];
+              const uint32_t a0 = w0 & 0x0f0f0f0fu, a2 = w0 >> 4 & 0x0f0f0f0fu;
+              const uint32_t a1 = w1 & 0x0f0f0f0fu, a3 = w1 >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_16832(part[r][n], a0, a1, a2, a3, b[n][2 * i], b[n][2 * i + 1]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[r][n][i] = fmaf(__int_as_float(part[r][n][i]) - __int_as_float(kMagic), sc[r][i >> 1] * f[n][i & 1],
+                                  acc[r][n][i]);
+      } else {
+        uint32_t zh[R][2];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) zh[r][h] = Nibbles<T>::high(zc[r][h]);
+        float part[R][NT][4];
+#pragma unroll
+        for (int j = 0; j < WPL; ++j) {
+          uint4 b[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            b[n] = *reinterpret_cast<const uint4*>(xp[n]);
+            xp[n] += x_step[n];
+          }
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            uint32_t lo[4], hi[4];
+            Nibbles<T>::decode(w[r][0][j], zc[r][0], zh[r][0], lo);
+            Nibbles<T>::decode(w[r][1][j], zc[r][1], zh[r][1], hi);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              if (j == 0) dev::mma_16816_zero<T>(part[r][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
+              else dev::mma_16816<T>(part[r][n], lo[0], hi[0], lo[1], hi[1], b[n].x, b[n].y);
+              dev::mma_16816<T>(part[r][n], lo[2], hi[2], lo[3], hi[3], b[n].z, b[n].w);
+            }
           }
         }
-      }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float f0 = 1.f, f1 = 1.f;  // x scales of the lane's two rows of x
-        if (XG) {
-          const int m = n * 8 + 2 * t;
-          f0 = m < p.mp ? sxs[(in_panel + s) * p.mp + m] : 0.f;
-          f1 = m + 1 < p.mp ? sxs[(in_panel + s) * p.mp + m + 1] : 0.f;
-        }
+        for (int n = 0; n < NT; ++n) {
+          float f0 = 1.f, f1 = 1.f;  // x scales of the lane's two rows of x
+          if (XG) {
+            const int m = n * 8 + 2 * t;
+            f0 = m < p.cols ? sxs[(in_panel + s) * p.cols + m] : 0.f;
+            f1 = m + 1 < p.cols ? sxs[(in_panel + s) * p.cols + m + 1] : 0.f;
+          }
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          acc[r][n][0] = fmaf(part[r][n][0], XG ? sc[r][0] * f0 : sc[r][0], acc[r][n][0]);
-          acc[r][n][1] = fmaf(part[r][n][1], XG ? sc[r][0] * f1 : sc[r][0], acc[r][n][1]);
-          acc[r][n][2] = fmaf(part[r][n][2], XG ? sc[r][1] * f0 : sc[r][1], acc[r][n][2]);
-          acc[r][n][3] = fmaf(part[r][n][3], XG ? sc[r][1] * f1 : sc[r][1], acc[r][n][3]);
+          for (int r = 0; r < R; ++r) {
+            acc[r][n][0] = fmaf(part[r][n][0], XG ? sc[r][0] * f0 : sc[r][0], acc[r][n][0]);
+            acc[r][n][1] = fmaf(part[r][n][1], XG ? sc[r][0] * f1 : sc[r][0], acc[r][n][1]);
+            acc[r][n][2] = fmaf(part[r][n][2], XG ? sc[r][1] * f0 : sc[r][1], acc[r][n][2]);
+            acc[r][n][3] = fmaf(part[r][n][3], XG ? sc[r][1] * f1 : sc[r][1], acc[r][n][3]);
+          }
         }
       }
     }
@@ -451,35 +635,47 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
 
     // the tile's sums
     auto store = [&](int m, int row, float y) {
-      if (!XG && a.x_scales) y *= a.x_scales[m];
+      if (a.x_scales && a.x_group >= a.k) y *= a.x_scales[m];
       const int64_t at = m * a.ldy + row;
       if (a.y_dtype == kDtF32) static_cast<float*>(a.y)[at] = y;
       else if (a.y_dtype == kDtBF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(y);
       else static_cast<__half*>(a.y)[at] = __float2half_rn(y);
     };
     const bool alone = p.wk == 1 && p.splits == 1;  // no other warp has a part of them
-    float* mine = red + (turn++ & 1) * (p.wk * COLS * block_rows);
+    float* mine = red + (turn++ & 1) * (p.wk * a.m * block_rows);
+    auto give = [&](int m, int row, float y) {
+      if (m >= a.m) return;
+      if (!alone) mine[(ks * a.m + m) * block_rows + row] = y;
+      else if (tile * block_rows + row < a.n) store(m, tile * block_rows + row, y);
+    };
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        const int row = wr * ROWS + r * 16 + g;
+        if (DIGITS && a.x_dtype != kDtI8) {
+          // the four digits of a row of x: two here, two in the next lane
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int m = n * 8 + 2 * t + (i & 1), row = wr * ROWS + r * 16 + (i >> 1) * 8 + g;
-          if (m < a.m) {
-            if (!alone) mine[(ks * COLS + m) * block_rows + row] = acc[r][n][i];
-            else if (tile * block_rows + row < a.n) store(m, tile * block_rows + row, acc[r][n][i]);
+          for (int h = 0; h < 2; ++h) {
+            float y = acc[r][n][2 * h] + acc[r][n][2 * h + 1];
+            y += __shfl_xor_sync(0xffffffffu, y, 1);
+            if (!(t & 1)) give(n * 2 + t / 2, row + h * 8, y);
           }
-          acc[r][n][i] = 0.f;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) give(n * 8 + 2 * t + (i & 1), row + (i >> 1) * 8, acc[r][n][i]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
+      }
     if (alone) continue;
     // over the warps, then over the cluster's panels, both in order; the buffers
     // alternate, so the next tile's sums need no second barrier
     __syncthreads();
     for (int i = threadIdx.x; i < a.m * block_rows; i += kThreads) {
       float v = 0.f;
-      for (int w = 0; w < p.wk; ++w) v += mine[w * COLS * block_rows + i];
-      if (p.splits > 1) mine[i] = v;  // [COLS][block_rows], over slice 0's part
+      for (int w = 0; w < p.wk; ++w) v += mine[w * a.m * block_rows + i];
+      if (p.splits > 1) mine[i] = v;  // over slice 0's part
       else if (tile * block_rows + i % block_rows < a.n) store(i / block_rows, tile * block_rows + i % block_rows, v);
     }
     if (p.splits > 1) {
@@ -515,9 +711,12 @@ cudaError_t launch_kernel(const W4Plan& p, size_t smem, cudaStream_t s) {
 
 template <typename T, int SEG, int R>
 cudaError_t launch_r(const W4Plan& p, bool xg, size_t smem, cudaStream_t s) {
-  if (p.mp <= 8)
+  if constexpr (std::is_same<T, int8_t>::value)
+    return p.cols <= 8 ? launch_kernel<T, SEG, R, 1, true>(p, smem, s) : launch_kernel<T, SEG, R, 2, true>(p, smem, s);
+  else if (p.cols <= 8)
     return xg ? launch_kernel<T, SEG, R, 1, true>(p, smem, s) : launch_kernel<T, SEG, R, 1, false>(p, smem, s);
-  return xg ? launch_kernel<T, SEG, R, 2, true>(p, smem, s) : launch_kernel<T, SEG, R, 2, false>(p, smem, s);
+  else
+    return xg ? launch_kernel<T, SEG, R, 2, true>(p, smem, s) : launch_kernel<T, SEG, R, 2, false>(p, smem, s);
 }
 
 template <typename T>
@@ -531,59 +730,78 @@ cudaError_t launch_seg(const W4Plan& p, int seg, int r, bool xg, size_t smem, cu
 }  // namespace
 
 cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s) {
-  W4Plan p = {};
-  p.a = a;
   const bool xg = a.x_scales && a.x_group < a.k;
-  if (!a.x_scales || !xg) p.a.x_group = a.k;
   const int seg = xg && a.x_group < a.group ? a.x_group : a.group;
-  p.segs = a.k / seg;
-  p.mp = a.m <= 1 ? 1 : a.m <= 2 ? 2 : a.m <= 4 ? 4 : a.m <= 8 ? 8 : 16;
-  const int nt = p.mp == 16 ? 2 : 1;
-  // A panel's rows of x take at most 48 KB of shared memory; a multiple of the
-  // weight group, so that no group is split over panels.
-  int panel_k = 48 * 1024 / 2 / p.mp;
-  int panels = (a.k + panel_k - 1) / panel_k;
-  panel_k = ((a.k + panels - 1) / panels + a.group - 1) / a.group * a.group;  // panels of one length
-  p.panels = (a.k + panel_k - 1) / panel_k;
-  p.splits = p.panels < 8 ? p.panels : 8;
-  p.panel_segs = panel_k / seg;
-  auto smem_of = [&](int r, int stages) {
-    const int stage_bytes = 16 * r * (kPitch + (kChunk / seg + (seg < 128 ? 1 : 0)) * 8);
-    size_t off = (size_t)kWarps * stages * stage_bytes;
-    p.off_x = (int)((off + 127) / 128 * 128);
-    off = p.off_x + (size_t)p.mp * panel_k * 2;
-    p.off_xs = (int)off;
-    if (xg) off += (size_t)p.panel_segs * p.mp * 4;
-    p.off_zero = (int)((off + 15) / 16 * 16);
-    p.off_red = p.off_zero + 16;
-    return p.off_red + (size_t)2 * kWarps * 8 * nt * 16 * r * 4;
-  };
-  // The shape (16 or 32 rows a warp, slices of a panel) with the least modelled
-  // time: rounds of blocks over the SMs, times the chunks of a slice (16 rows
-  // take 0.6 of the time of 32) plus a tile's sums (a third of a chunk; two
-  // chunks with a cluster's barriers).
-  double best = 0;
-  int r = 0;
-  for (int rr = 1; rr <= 2; ++rr) {
-    // three stages where two blocks still fit an SM, or two
-    const int stages = smem_of(rr, 3) <= kSmemLimit / 2 ? 3 : 2;
-    const size_t bytes = smem_of(rr, stages);
-    if (bytes > kSmemLimit) continue;
-    const int resident = (bytes <= kSmemLimit / 2 ? 2 : 1) * 148 / p.splits;
-    for (int wk = 1; wk <= 8; wk *= 2) {
-      const int64_t block_rows = 16LL * rr * (8 / wk), tiles = (a.n + block_rows - 1) / block_rows;
-      const int slice = (p.panel_segs + wk - 1) / wk, chunks = (slice * seg + kChunk - 1) / kChunk;
-      const double cost = (double)((tiles + resident - 1) / resident) *
-                          (chunks * (rr == 1 ? 0.6 : 1.0) + (p.splits > 1 ? 2.0 : 0.35));
-      if (r && cost >= best) continue;
-      best = cost, r = rr;
-      p.wk = wk, p.slice_segs = slice, p.tiles = (int)tiles, p.stages = stages;
-      p.blocks = p.tiles < resident ? p.tiles : resident;
+  W4Plan best = {};
+  double best_cost = 0;
+  size_t best_smem = 0;
+  int best_r = 0;
+  bool best_digits = false;
+  // Digits or floating point, 16 or 32 rows a warp, slices of a panel: whatever
+  // has the least modelled time. That is the rounds of blocks over the SMs,
+  // times the chunks of a slice (1 with 32 rows, 0.6 with 16; digits cost less
+  // of it the longer the segments are) plus a tile's sums (a third of a chunk;
+  // two chunks with a cluster's barriers), plus a block's preparation of digits
+  // for each eight elements a thread prepares. One f16 row, group 128, us with
+  // digits and without: 131072 x 2048 29 / 38, 5120 x 2048 4.8 / 5.0, 2048 x 6144
+  // 7.1 / 6.6; group 64, 6144 x 6144: 14.9 / 10.7; sixteen i8 rows, 131072 x 2048
+  // 62 / 87, 5120 x 2048 15.5 / 11.2. Digits take four columns a row of x, so
+  // they are for two rows at most (four rows against 131072 x 2048: 50 us, 42
+  // without) and for i8, where they are one.
+  const double digit_chunk = seg == 128 ? 0.8 : seg == 64 ? 1.0 : 1.2;
+  for (int digits = 0; digits < (a.x_dtype == kDtI8 || a.m <= 2 ? 2 : 1); ++digits) {
+    W4Plan p = {};
+    p.a = a;
+    if (!xg) p.a.x_group = a.k;
+    p.segs = a.k / seg;
+    p.cols = digits ? (a.x_dtype == kDtI8 ? (a.m + 1) / 2 * 2 : 4 * a.m)
+                    : a.m <= 1 ? 1 : a.m <= 2 ? 2 : a.m <= 4 ? 4 : a.m <= 8 ? 8 : 16;
+    const int x_bytes = digits ? p.cols : 2 * p.cols;  // of a column of the weights
+    // A panel's rows of x take at most 48 KB of shared memory; a multiple of the
+    // weight group, so that no group is split over panels.
+    int panel_k = 48 * 1024 / x_bytes;
+    const int panels = (a.k + panel_k - 1) / panel_k;
+    panel_k = ((a.k + panels - 1) / panels + a.group - 1) / a.group * a.group;  // panels of one length
+    p.panels = (a.k + panel_k - 1) / panel_k;
+    p.splits = p.panels < 8 ? p.panels : 8;
+    p.panel_segs = panel_k / seg;
+    auto smem_of = [&](int r, int stages) {
+      const int stage_bytes = 16 * r * (kPitch + (kChunk / seg + (seg < 128 ? 1 : 0)) * 8);
+      size_t off = (size_t)kWarps * stages * stage_bytes;
+      p.off_x = (int)((off + 127) / 128 * 128);
+      off = p.off_x + (size_t)panel_k * x_bytes;
+      p.off_xs = (int)off;
+      if (xg || digits) off += (size_t)p.panel_segs * p.cols * (digits ? 8 : 4);
+      p.off_zero = (int)((off + 15) / 16 * 16);
+      p.off_red = p.off_zero + 16;
+      return p.off_red + (size_t)2 * kWarps * a.m * 16 * r * 4;
+    };
+    // of a block: a thread's eight elements each, more for four digits
+    const double prepare = digits ? (double)a.m * panel_k / 8 / kThreads * (a.x_dtype == kDtI8 ? 0.16 : 0.15) : 0;
+    for (int r = 1; r <= 2; ++r) {
+      // three stages where two blocks still fit an SM, or two
+      p.stages = smem_of(r, 3) <= kSmemLimit / 2 ? 3 : 2;
+      const size_t bytes = smem_of(r, p.stages);
+      if (bytes > kSmemLimit) continue;
+      const int resident = (bytes <= kSmemLimit / 2 ? 2 : 1) * 148 / p.splits;
+      for (p.wk = 1; p.wk <= 8; p.wk *= 2) {
+        const int64_t block_rows = 16LL * r * (8 / p.wk), tiles = (a.n + block_rows - 1) / block_rows;
+        p.slice_segs = (p.panel_segs + p.wk - 1) / p.wk;
+        const int chunks = (p.slice_segs * seg + kChunk - 1) / kChunk;
+        const double cost = (double)((tiles + resident - 1) / resident) *
+                                (chunks * (r == 1 ? 0.6 : 1.0) * (digits ? digit_chunk : 1.0) + (p.splits > 1 ? 2.0 : 0.35)) +
+                            prepare;
+        if (best_r && cost >= best_cost) continue;
+        p.tiles = (int)tiles;
+        p.blocks = p.tiles < resident ? p.tiles : resident;
+        best = p, best_cost = cost, best_smem = bytes, best_r = r, best_digits = digits;
+      }
     }
   }
-  if (!r) return cudaErrorInvalidValue;
-  const size_t off = smem_of(r, p.stages);
-  return a.x_dtype == kDtBF16 ? launch_seg<__nv_bfloat16>(p, seg, r, xg, off, s) : launch_seg<__half>(p, seg, r, xg, off, s);
+  if (!best_r) return cudaErrorInvalidValue;
+  if (best_digits) return launch_seg<int8_t>(best, seg, best_r, xg, best_smem, s);
+  return a.x_dtype == kDtBF16 ? launch_seg<__nv_bfloat16>(best, seg, best_r, xg, best_smem, s)
+                              : launch_seg<__half>(best, seg, best_r, xg, best_smem, s);
 }
 
 }  // namespace nemo

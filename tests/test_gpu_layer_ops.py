@@ -170,6 +170,46 @@ def test_w4_matvec_rows_longer_than_a_cluster_holds(gen, xt, group, x_group, m, 
     ref.check_w4(x, xs, x_group, q, s, z, group, y, F32)
 
 
+@pytest.mark.parametrize("xt,group,x_group,m,n,k", [
+    (F16, 128, 0, 1, 20000, 1024), (BF16, 128, 0, 2, 60000, 640), (E4M3, 128, 128, 1, 30000, 2176),
+    (F16, 64, 0, 1, 90000, 576), (F16, 32, 0, 1, 90000, 288), (E4M3, 128, 32, 2, 70000, 512), (I8, 128, 128, 1, 9001, 1024),
+    (I8, 128, 0, 5, 40000, 384), (I8, 64, 32, 16, 60000, 256), (I8, 32, 10 ** 6, 3, 50000, 160),
+    (F16, 128, 0, 1, 4000, 65536)])
+def test_w4_matvec_many_rows(gen, xt, group, x_group, m, n, k):
+    x, xs, q, s, z = w4_inputs(gen, xt, m, n, k, group, True, F16, x_group or k)
+    y = ref.w4_matvec(x, xs, x_group or k, ref.pack4(q), s, ref.pack4(z), group, n, F32)
+    ref.check_w4(x, xs, x_group or k, q, s, z, group, y, F32)
+
+
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("xt,shift", [(F16, 0), (BF16, 0), (BF16, 100), (BF16, -70), (E4M3, 0)])
+def test_w4_matvec_many_rows_of_uneven_values(gen, xt, shift, m):
+    """Elements of a row whose magnitudes differ by 2^20 or more, whole groups of zeros and lone elements."""
+    n, k, group = 50000, 1024, 128
+    x, xs, q, s, z = w4_inputs(gen, xt, m, n, k, group, True, F16, k)
+    spread = torch.randint(-10, 11, (m, k), generator=gen, device="cuda").double()
+    if xt == E4M3:
+        x = (x.float() * 2.0 ** (spread.float() - 10)).clamp(-448, 448).to(TORCH[xt])
+    else:
+        x = (x.double() * 2.0 ** (spread + shift)).clamp(-60000 * 2.0 ** shift, 60000 * 2.0 ** shift).to(TORCH[xt])
+    x.view(torch.uint8 if xt == E4M3 else torch.int16)[:, 128:256] = 0
+    x.view(torch.uint8 if xt == E4M3 else torch.int16)[:, 300:384] = 0
+    y = ref.w4_matvec(x, xs, k, ref.pack4(q), s, ref.pack4(z), group, n, F32)
+    ref.check_w4(x, xs, k, q, s, z, group, y, F32)
+
+
+def test_w4_matvec_many_rows_do_not_mix(gen):
+    m, n, k = 2, 50000, 512
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        x, _, q, s, _ = w4_inputs(gen, BF16, m, n, k, 128, False, F16, k)
+        x[1, 300] = bad
+        s[7, 0] = float("inf")
+        y = ref.w4_matvec(x, None, 0, ref.pack4(q), s, None, 128, n, F32)
+        want = torch.zeros((m, n), dtype=torch.bool, device="cuda")
+        want[1], want[:, 7] = True, True
+        assert torch.equal(~torch.isfinite(y), want)
+
+
 def test_w4_matvec_strides_and_odd_addresses(gen):
     m, n, k = 6, 50, 512
     x, _, q, s, z = w4_inputs(gen, F16, m, n, k, 64, True, F16, k)
