@@ -203,6 +203,19 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
+// A row of x and one of its units of eight elements. A block's threads walk over
+// the units of all rows in order: one division each at the start.
+struct Unit {
+  int units, rows_on, units_on;  // of a row; a step of the block
+  int m, u;
+  __device__ __forceinline__ Unit(int units_, int thread)
+      : units(units_), rows_on(kThreads / units_), units_on(kThreads % units_), m(thread / units_), u(thread % units_) {}
+  __device__ __forceinline__ void advance() {
+    m += rows_on, u += units_on;
+    if (u >= units) u -= units, ++m;
+  }
+};
+
 // T: type of the products (f16 also for 8-bit x, which it holds exactly; int8_t:
 // digits). R: 16-row tiles per warp. NT: 8-column tiles of x's operand. XG: x
 // scales per group (always with digits).
@@ -231,6 +244,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
   const int seg_shift = a.group == SEG ? 0 : a.group == 2 * SEG ? 1 : 2;  // segments of a group, log2
   const int zero_bytes = (groups + 1) / 2;
   const int x_groups = (a.k + a.x_group - 1) / a.x_group;
+  const int x_shift = 31 - __clz(a.x_group);  // (a power of two where there is more than one)
   const int64_t row_bytes = a.k / 2;
 
   // The warp's chunks in order: tiles blockIdx.x, + gridDim.x, ...; of each, the
@@ -335,17 +349,16 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
     const int seg0 = panel * p.panel_segs, n = min(p.panel_segs, p.segs - seg0);
     const int units = n * (SEG / 8);  // of a row
     constexpr int kAhead = 4;         // loads in flight
-    for (int i0 = threadIdx.x; i0 < p.cols * units; i0 += kAhead * kThreads) {
+    Unit at(units, threadIdx.x);
+    while (at.m < p.cols) {
       uint4 raw[kAhead];
       int to[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int i = i0 + j * kThreads;
-        const int m = i / units, u = i - m * units;
-        const int seg = u / (SEG / 8), rem = u % (SEG / 8);
-        to[j] = i < p.cols * units ? (((seg * WPL + rem % WPL) * p.cols + m) * 4 + rem / WPL) * 16 : -1;
+      for (int j = 0; j < kAhead; ++j, at.advance()) {
+        const int seg = at.u / (SEG / 8), rem = at.u % (SEG / 8);
+        to[j] = at.m < p.cols ? (((seg * WPL + rem % WPL) * p.cols + at.m) * 4 + rem / WPL) * 16 : -1;
         raw[j] = make_uint4(0, 0, 0, 0);
-        if (m < a.m && i < p.cols * units) raw[j] = load_x8<CODES>(a.x, m * a.ldx + (int64_t)seg0 * SEG + u * 8);
+        if (at.m < a.m) raw[j] = load_x8<CODES>(a.x, at.m * a.ldx + (int64_t)seg0 * SEG + at.u * 8);
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j)
@@ -354,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
     if (XG)
       for (int i = threadIdx.x; i < n * p.cols; i += kThreads) {
         const int m = i % p.cols, seg = i / p.cols;
-        sxs[i] = m < a.m ? a.x_scales[(int64_t)m * x_groups + (int64_t)(seg0 + seg) * SEG / a.x_group] : 0.f;
+        sxs[i] = m < a.m ? a.x_scales[(int64_t)m * x_groups + ((seg0 + seg) * SEG >> x_shift)] : 0.f;
       }
   };
   // The same as digits: element x of a segment whose largest magnitude is below
@@ -370,24 +383,25 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
     const int seg0 = panel * p.panel_segs, n = min(p.panel_segs, p.segs - seg0);
     const int units = n * LANES, rows = KIND == kDtI8 ? p.cols : a.m;
     constexpr int kAhead = 4;
-    for (int m = 0; m < rows; ++m)
-    for (int u0 = threadIdx.x - lane; u0 < units; u0 += kAhead * kThreads) {  // (of the warp)
+    // every lane of a warp takes part in the segments' sums until its warp is done
+    Unit from(units, threadIdx.x);
+    while (__any_sync(0xffffffffu, from.m < rows)) {
       uint4 raw[kAhead];
+      Unit of = from;
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int u = u0 + j * kThreads + lane;
+      for (int j = 0; j < kAhead; ++j, of.advance()) {
         raw[j] = make_uint4(0, 0, 0, 0);
-        if (u < units && m < a.m) raw[j] = load_x8<CODES>(a.x, m * a.ldx + (int64_t)seg0 * SEG + u * 8);
+        if (of.m < a.m) raw[j] = load_x8<CODES>(a.x, of.m * a.ldx + (int64_t)seg0 * SEG + of.u * 8);
       }
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        if (u0 + j * kThreads >= units) break;
-        const int u = u0 + j * kThreads + lane;
+      for (int j = 0; j < kAhead; ++j, from.advance()) {
+        if (!__any_sync(0xffffffffu, from.m < rows)) break;
+        const int m = from.m, u = from.u;
+        const bool in = m < rows;
         const int seg = u / LANES, rem = u % LANES, word = rem % WPL;
-        const bool in = u < units;
         float xs = 1.f;
         if (in && a.x_group < a.k)
-          xs = m < a.m ? a.x_scales[(int64_t)m * x_groups + (int64_t)(seg0 + seg) * SEG / a.x_group] : 0.f;
+          xs = m < a.m ? a.x_scales[(int64_t)m * x_groups + ((seg0 + seg) * SEG >> x_shift)] : 0.f;
         const int at = (seg * (WPL / XW) + word / XW) * p.cols;  // the columns' rows of 4 lanes
         uint8_t* to = sx + (rem / WPL) * (XW * 8) + word % XW * 8;
         if constexpr (KIND == kDtI8) {
@@ -744,8 +758,8 @@ cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s) {
   // two chunks with a cluster's barriers), plus a block's preparation of digits
   // for each eight elements a thread prepares. One f16 row, group 128, us with
   // digits and without: 131072 x 2048 29 / 38, 5120 x 2048 4.8 / 5.0, 2048 x 6144
-  // 7.1 / 6.6; group 64, 6144 x 6144: 14.9 / 10.7; sixteen i8 rows, 131072 x 2048
-  // 62 / 87, 5120 x 2048 15.5 / 11.2. Digits take four columns a row of x, so
+  // 7.4 / 6.6; group 64, 6144 x 6144: 14.8 / 10.7; sixteen i8 rows, 131072 x 2048
+  // 59 / 83, 5120 x 2048 11.4 / 11.0. Digits take four columns a row of x, so
   // they are for two rows at most (four rows against 131072 x 2048: 50 us, 42
   // without) and for i8, where they are one.
   const double digit_chunk = seg == 128 ? 0.8 : seg == 64 ? 1.0 : 1.2;
@@ -777,7 +791,7 @@ cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s) {
       return p.off_red + (size_t)2 * kWarps * a.m * 16 * r * 4;
     };
     // of a block: a thread's eight elements each, more for four digits
-    const double prepare = digits ? (double)a.m * panel_k / 8 / kThreads * (a.x_dtype == kDtI8 ? 0.16 : 0.15) : 0;
+    const double prepare = digits ? (double)a.m * panel_k / 8 / kThreads * (a.x_dtype == kDtI8 ? 0.04 : 0.15) : 0;
     for (int r = 1; r <= 2; ++r) {
       // three stages where two blocks still fit an SM, or two
       p.stages = smem_of(r, 3) <= kSmemLimit / 2 ? 3 : 2;
