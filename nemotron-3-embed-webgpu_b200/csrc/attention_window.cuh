@@ -99,7 +99,7 @@ __device__ __noinline__ void attention_row(const AttnWindowArgs& a, AttnRequest 
         acc[c] = acc[c] * keep + w * dev::to_f32(v[(int64_t)j * a.ldv + c * 32 + lane]);
         lost &= isnan(acc[c]);
       }
-    if (__all_sync(0xffffffffu, lost)) break;  // every column is NaN: no later key changes that
+    if (l > 0.f && __all_sync(0xffffffffu, lost)) break;  // every column is NaN: no later key changes that
     m = mn;
   }
   T* out = static_cast<T*>(a.out) + (int64_t)(r.q0 + i) * a.ldo + head * d;

@@ -225,6 +225,18 @@ def test_w4_matvec_strides_and_odd_addresses(gen):
     ref.check_w4(bytes_x[:, 1:k + 1], xs, 128, q, s, z, 64, y, F32)
 
 
+@pytest.mark.parametrize("xt,m", [(F16, 2), (E4M3, 1), (I8, 3)])
+def test_w4_matvec_many_rows_from_odd_addresses(gen, xt, m):
+    n, k = 40000, 512
+    x, xs, q, s, z = w4_inputs(gen, xt, m, n, k, 128, True, F16, k)
+    wide = torch.zeros((m, k + 5), dtype=TORCH[xt], device="cuda")
+    wide[:, 3:k + 3] = x
+    y = torch.full((m, n + 3), 9.0, device="cuda")
+    ref.w4_matvec(wide[:, 3:k + 3], xs, k, ref.pack4(q), s, ref.pack4(z), 128, n, F32, y=y[:, :n])
+    ref.check_w4(x, xs, k, q, s, z, 128, y[:, :n], F32)
+    assert (y[:, n:] == 9.0).all()
+
+
 def test_w4_matvec_rows_do_not_mix(gen):
     """A NaN in one row of x and an infinite scale in one row of W stay in theirs."""
     m, n, k = 4, 64, 256
@@ -377,6 +389,17 @@ def test_attention_window_nothing_but_bad_values(gen, dt, q_len, hq):
         vv = v if values is None else torch.full_like(v, values)
         got = ref.attention(q, kk, vv, *args[3:], 300, 0, 2)
         assert (got == 0).all() if keys == -float("inf") else torch.isnan(got).all()
+
+
+@pytest.mark.parametrize("q_len,hq", [(1, 2), (200, 2), (1200, 8)])
+def test_attention_window_nan_values_of_keys_without_weight(gen, q_len, hq):
+    """A score of -infinity is a weight of 0, and 0 times a NaN is a NaN, wherever among the keys it stands."""
+    for at in (0, 1199):
+        args = packed(gen, F16, [q_len], [1200], hq, 1, 64)
+        q, k, v = args[:3]
+        q.abs_().add_(0.5)
+        k[at], v[at] = -float("inf"), float("nan")
+        assert torch.isnan(ref.attention(*args, -1, -1, 0)).all()
 
 
 @pytest.mark.parametrize("longest", [40, 900])
