@@ -422,7 +422,16 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
           for (int c = 0; c < 8; ++c) top = max(top, __float_as_uint(v[c]) & 0x7fffffffu);
 #pragma unroll
           for (int o = 1; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int e = max((int)(top >> 23) - 127, -97);  // 2^(29 - e) and its inverse are normal
+          int e = (int)(top >> 23) - 127;
+          // A factor 2^(29 - e) is finite from e = -97 on. bf16 goes on below: such segments are raised
+          // by 2^23 first, to at least 2^-97 or all of them whole multiples of the unit 2^-149.
+          const bool raised = KIND == kDtBF16 && e < -97;
+          if (raised) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] *= 8388608.f;
+            e += 23;
+          }
+          e = max(e, -97);
           const float up = __uint_as_float((uint32_t)(156 - e) << 23);
           uint32_t d[8];
 #pragma unroll
@@ -454,8 +463,9 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
               const int pair = rem & 2 ? high : low, first = (int16_t)(pair & 0xffff);
               sums[seg * p.cols + 4 * m + rem] = rem & 1 ? (pair - first) >> 16 : first;
               // an infinity or NaN makes every product of the row NaN
-              sxs[seg * p.cols + 4 * m + rem] =
-                  top < 0x7f800000u ? xs * __uint_as_float((uint32_t)(e + 98 + 8 * rem) << 23) : __uint_as_float(0x7fc00000u);
+              float unit = __uint_as_float((uint32_t)(e + 98 + 8 * rem) << 23);
+              if (raised) unit *= 1.f / 8388608.f;  // (exact, if subnormal)
+              sxs[seg * p.cols + 4 * m + rem] = top < 0x7f800000u ? xs * unit : __uint_as_float(0x7fc00000u);
             }
           }
         }
@@ -591,7 +601,8 @@ __global__ void __launch_bounds__(kThreads, 2) w4_matvec_kernel(const __grid_con
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              acc[r][n][i] = fmaf(__int_as_float(part[r][n][i]) - __int_as_float(kMagic), sc[r][i >> 1] * f[n][i & 1],
+              // (the unit of the digit first: exact for 16-bit x, and its product with a weight's scale may underflow)
+              acc[r][n][i] = fmaf((__int_as_float(part[r][n][i]) - __int_as_float(kMagic)) * f[n][i & 1], sc[r][i >> 1],
                                   acc[r][n][i]);
       } else {
         uint32_t zh[R][2];
