@@ -59,54 +59,182 @@ struct KeyRange {
   }
 };
 
-// The output of query row i of request r for one head, columns [d0, d1), by one
-// warp, key by key and touching only keys that the query sees. The tiled
-// kernels multiply weights of 0 with values of keys that other queries of the
-// tile see; where such a value is infinite or NaN the product is NaN, and the
-// rows it reached are computed again here (up to the key that settles the row,
-// so that a call on NaN throughout does not crawl).
+// Which of 8 elements have an exponent field of ones (an infinity or NaN), and
+// which are NaN: a bit each.
 template <typename T>
-__device__ __noinline__ void attention_row(const AttnWindowArgs& a, AttnRequest r, int i, int head, int d0,
-                                           int d1) {
-  const int lane = threadIdx.x & 31, d = a.head_dim;
+struct Special;
+template <>
+struct Special<__half> {
+  static constexpr uint32_t kExp = 0x7c00;
+};
+template <>
+struct Special<__nv_bfloat16> {
+  static constexpr uint32_t kExp = 0x7f80;
+};
+template <typename T>
+__device__ __forceinline__ bool any_special(const uint4& u) {
+  constexpr uint32_t kExp2 = Special<T>::kExp * 0x10001u, kStep = (0x8000u - Special<T>::kExp) * 0x10001u;
+  return ((((u.x & kExp2) + kStep) | ((u.y & kExp2) + kStep) | ((u.z & kExp2) + kStep) | ((u.w & kExp2) + kStep)) &
+          0x80008000u) != 0;
+}
+template <typename T>
+__device__ __forceinline__ void special8(const uint4& u, uint32_t& nans, uint32_t& infs) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  nans = infs = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t h = w[e / 2] >> (e & 1) * 16 & 0x7fff;
+    nans |= (h > Special<T>::kExp ? 1u : 0u) << e;
+    infs |= (h == Special<T>::kExp ? 1u : 0u) << e;
+  }
+}
+
+// The elements of columns 8 g .. 8 g + 7 of a head's values (v) that are NaN or
+// infinite in some key of `range`, as bits; by one warp, a key a lane. Ends once
+// every column of `want` has a NaN, or an infinity where `inf_will_do`.
+template <typename T>
+__device__ __forceinline__ void seen_specials(const T* v, int64_t ldv, const KeyRange& range, int g, uint32_t want,
+                                              uint32_t inf_will_do, uint32_t& nans, uint32_t& infs) {
+  constexpr int kAhead = 4;
+  const int lane = threadIdx.x & 31;
+  nans = infs = 0;
+  for (int part = 0; part < 2; ++part) {
+    const int end = part ? range.hi : range.sink;
+    for (int j = part ? range.lo : 0; j < end; j += 32 * kAhead) {
+      uint4 u[kAhead];
+      bool hit = false;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int key = j + i * 32 + lane;
+        u[i] = make_uint4(0, 0, 0, 0);
+        if (key < end) u[i] = *reinterpret_cast<const uint4*>(v + (int64_t)key * ldv + g * 8);
+        hit |= any_special<T>(u[i]);
+      }
+      if (!__any_sync(0xffffffffu, hit)) continue;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        uint32_t n, f;
+        special8<T>(u[i], n, f);
+        nans |= __reduce_or_sync(0xffffffffu, n);
+        infs |= __reduce_or_sync(0xffffffffu, f);
+      }
+      if (!(want & ~nans & ~(infs & inf_will_do))) return;
+    }
+  }
+}
+
+// Makes the columns [d0, d1) of the output of query row i of request r for one
+// head right where the tiled kernels left an infinity or NaN there, by one warp.
+// Those kernels multiply weights of 0 with values of keys that other queries of
+// the tile see, so a value that is infinite or NaN reaches rows that do not see
+// it. Only called where the row's sum of weights is finite, that is where no
+// score of a key that it sees is NaN or +infinity. A column stands as it is if
+// the row does see a NaN in it, or, where the result is an infinity (and so no
+// NaN arose), sees an infinity: that takes one walk over the column's values.
+// What is left is computed again from the keys that the row sees, 32 at a time.
+// (8192 causal queries of 24 heads of 128 with one such value in sight of all: a
+// walk key by key over every row took 228 ms where the clean call takes 0.4.)
+template <typename T, int D>
+__device__ __noinline__ void attention_row(const AttnWindowArgs& a, AttnRequest r, int i, int head, int d0, int d1) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int kLanes = D / 8;         // lanes with 8 columns each
+  constexpr int kKeys = 32 / kLanes;    // keys side by side
+  const int lane = threadIdx.x & 31, g = lane % kLanes, sub = lane / kLanes;
   const int kvh = head / (a.q_heads / a.kv_heads);
   const int p = i + r.nk - r.nq;
-  const T* q = static_cast<const T*>(a.q) + (int64_t)(r.q0 + i) * a.ldq + head * d;
-  const T* k = static_cast<const T*>(a.k) + (int64_t)r.k0 * a.ldk + kvh * d;
-  const T* v = static_cast<const T*>(a.v) + (int64_t)r.k0 * a.ldv + kvh * d;
+  const T* q = static_cast<const T*>(a.q) + (int64_t)(r.q0 + i) * a.ldq + head * D;
+  const T* k = static_cast<const T*>(a.k) + (int64_t)r.k0 * a.ldk + kvh * D;
+  const T* v = static_cast<const T*>(a.v) + (int64_t)r.k0 * a.ldv + kvh * D;
+  T* out = static_cast<T*>(a.out) + (int64_t)(r.q0 + i) * a.ldo + head * D;
   const KeyRange range(a, p, p, r.nk);
-  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < range.hi; ++j) {
-    if (j == range.sink && range.lo > j) j = range.lo;
-    if (j >= range.hi) break;
-    float s = 0.f;
-    for (int c = lane; c < d; c += 32) s += dev::to_f32(q[c]) * dev::to_f32(k[(int64_t)j * a.ldk + c]);
+
+  uint32_t need = 0, inf_out = 0;  // of the lane's columns: to be looked at, infinite
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= a.scale * 1.4426950408889634f;
-    if (!(s < INFINITY)) {  // a NaN or +infinity score makes the row NaN, as it does in a softmax
-      l = __uint_as_float(0x7fc00000u);
-      break;
-    }
-    const float mn = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : exp2f(m - mn);
-    const float w = s == -INFINITY ? 0.f : exp2f(s - mn);
-    l = l * keep + w;
-    bool lost = true;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c * 32 + lane < d) {
-        acc[c] = acc[c] * keep + w * dev::to_f32(v[(int64_t)j * a.ldv + c * 32 + lane]);
-        lost &= isnan(acc[c]);
-      }
-    if (l > 0.f && __all_sync(0xffffffffu, lost)) break;  // every column is NaN: no later key changes that
-    m = mn;
+  for (int e = 0; e < 8; ++e) {
+    const int col = g * 8 + e;
+    if (col < d0 || col >= d1) continue;
+    const uint32_t h = *reinterpret_cast<const uint16_t*>(out + col) & 0x7fff;
+    need |= (h >= Special<T>::kExp ? 1u : 0u) << e;
+    inf_out |= (h == Special<T>::kExp ? 1u : 0u) << e;
   }
-  T* out = static_cast<T*>(a.out) + (int64_t)(r.q0 + i) * a.ldo + head * d;
+  for (uint32_t left = __ballot_sync(kAll, sub == 0 && need); left; left &= left - 1) {
+    const int from = __ffs(left) - 1;
+    const uint32_t want = __shfl_sync(kAll, need, from), inf_will_do = __shfl_sync(kAll, inf_out, from);
+    uint32_t nans, infs;
+    seen_specials<T>(v, a.ldv, range, from, want, inf_will_do, nans, infs);
+    if (g == from) need &= ~(nans | (infs & inf_out));
+  }
+  if (!__any_sync(kAll, need)) return;
+
+  float qv[8], m = -INFINITY, l = 0.f, acc[8];  // acc: the mean so far, of the lane's columns and keys
+  dev::unpack8<T>(*reinterpret_cast<const uint4*>(q + g * 8), qv);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int col = c * 32 + lane;
-    if (col >= d0 && col < d1) out[col] = dev::from_f32<T>(l == 0.f ? 0.f : acc[c] / l);
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  bool done = false;
+  for (int part = 0; part < 2 && !done; ++part) {
+    const int end = part ? range.hi : range.sink;
+    for (int base = part ? range.lo : 0; base < end && !done; base += 32) {
+      const int n = min(32, end - base);
+      float s = 0.f;
+#pragma unroll 8
+      for (int t = 0; t < kLanes; ++t) {
+        const int key = t * kKeys + sub;
+        float dot = 0.f;
+        if (key < n) {
+          float kv[8];
+          dev::unpack8<T>(*reinterpret_cast<const uint4*>(k + (int64_t)(base + key) * a.ldk + g * 8), kv);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dot = fmaf(qv[e], kv[e], dot);
+        }
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) dot += __shfl_xor_sync(kAll, dot, o);
+        const float x = __shfl_sync(kAll, dot, lane % kKeys * kLanes);
+        if (lane / kKeys == t) s = x;  // lane = key
+      }
+      s = lane < n ? s * (a.scale * 1.4426950408889634f) : -INFINITY;
+      if (__any_sync(kAll, !(s < INFINITY))) {  // makes the row NaN, as in a softmax
+        l = __uint_as_float(0x7fc00000u);
+        done = true;
+        break;
+      }
+      float mn = s, sum;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(kAll, mn, o));
+      mn = fmaxf(mn, m);
+      float w = s == -INFINITY ? 0.f : exp2f(s - mn);
+      sum = w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+      const float kept = m == -INFINITY ? 0.f : l * exp2f(m - mn);
+      m = mn, l = kept + sum;
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      w *= inv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= kept * inv;
+#pragma unroll 8
+      for (int t = 0; t < kLanes; ++t) {
+        const int key = t * kKeys + sub;
+        const float wk = __shfl_sync(kAll, w, key);
+        if (key < n && need) {
+          float vv[8];
+          dev::unpack8<T>(*reinterpret_cast<const uint4*>(v + (int64_t)(base + key) * a.ldv + g * 8), vv);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] = fmaf(wk, vv[e], acc[e]);
+        }
+      }
+      uint32_t lost = 0;  // columns that are NaN whatever follows
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lost |= (isnan(acc[e]) ? 1u : 0u) << e;
+#pragma unroll
+      for (int o = kLanes; o < 32; o <<= 1) lost |= __shfl_xor_sync(kAll, lost, o);
+      done = l > 0.f && __all_sync(kAll, !(need & ~lost));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+#pragma unroll
+    for (int o = kLanes; o < 32; o <<= 1) acc[e] += __shfl_xor_sync(kAll, acc[e], o);
+    if (sub == 0 && (need >> e & 1)) out[g * 8 + e] = dev::from_f32<T>(l == 0.f ? 0.f : l > 0.f ? acc[e] : l);
   }
 }
 

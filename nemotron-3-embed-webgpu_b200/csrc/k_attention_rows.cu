@@ -281,9 +281,14 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
       acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
     }
     if (global_row >= rows) continue;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-    if (!isfinite(acc.x + acc.y + acc.z + acc.w)) atomicOr(bad, 1u << row);
+    if (sum == 0.f) {
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+      const float inv = 1.f / sum;
+      acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+      // (a sum that is not finite is a score that is not: the row is NaN)
+      if (isfinite(sum) && !isfinite(acc.x + acc.y + acc.z + acc.w)) atomicOr(bad, 1u << row);
+    }
     const int qi = global_row / group, head = kvh * group + global_row % group;
     *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(rq.q0 + qi) * a.ldo + head * D + d0 + c) =
         make_uint2(dev::pack2<T>(acc.x, acc.y), dev::pack2<T>(acc.z, acc.w));
@@ -293,7 +298,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
   for (int n = 0; rest; ++n, rest &= rest - 1) {
     const int row = __ffs(rest) - 1, global_row = tile * 16 + row;
     if (n % kWarps == warp)
-      attention_row<T>(a, rq, global_row / group, kvh * group + global_row % group, d0, d1);
+      attention_row<T, D>(a, rq, global_row / group, kvh * group + global_row % group, d0, d1);
   }
 }
 

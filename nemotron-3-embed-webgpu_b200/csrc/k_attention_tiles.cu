@@ -62,7 +62,9 @@ struct TilesCfg {
   static constexpr int kStages = 4;              // K and V tiles in flight: two ahead of V for S, one to load
   static constexpr int kThreads = 384;
   static constexpr int kListedBytes = 96 * kListed;  // a Pair each
-  static constexpr int kSmem = 1024 + 2 * kQ + kStages * 2 * kTileBytes + 256 + kListedBytes + (kMaxRequests + 1) * 4;
+  static constexpr int kRedoBytes = 32 * kListed;    // a bit for each row of a Pair
+  static constexpr int kSmem =
+      1024 + 2 * kQ + kStages * 2 * kTileBytes + 256 + kListedBytes + kRedoBytes + (kMaxRequests + 1) * 4;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColS = 0, kColO = 256;  // S tile i of unit t at 128 t + 64 i, O_t at 256 + 128 t
 };
@@ -220,9 +222,10 @@ __global__ void __launch_bounds__(384, 1)
   const uint32_t s_full = q_full + 16, p_ready = s_full + 32, pv_done = p_ready + 32, mma_fin = pv_done + 32;
   const uint32_t kv_full = mma_fin + 8, kv_ready = kv_full + 8 * C::kStages, kv_empty = kv_ready + 8 * C::kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
-  uint32_t* bad = tmem_slot + 1;  // some output of this block is not finite
+  uint32_t* bad = tmem_slot + 1;  // some output of this block has to be looked at again
   Pair* listed = reinterpret_cast<Pair*>(bars + 32);
-  int* before = reinterpret_cast<int*>(bars + 32) + C::kListedBytes / 4;
+  uint32_t* redo = reinterpret_cast<uint32_t*>(bars + 32) + C::kListedBytes / 4;  // its rows: [item][unit][quarter]
+  int* before = reinterpret_cast<int*>(redo) + C::kRedoBytes / 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 0 && lane == 0) {
@@ -286,6 +289,7 @@ __global__ void __launch_bounds__(384, 1)
     const int item = mine.nth(threadIdx.x);
     if (item < total) listed[threadIdx.x] = mine.find(a, item);
   }
+  for (int i = threadIdx.x; i < C::kRedoBytes / 4; i += C::kThreads) redo[i] = 0;
   __syncthreads();
 
   if (warp == 0) {
@@ -598,7 +602,6 @@ __global__ void __launch_bounds__(384, 1)
         uint32_t v[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          // a row that has seen nothing has zeros there (0 times finite values) or garbage times inv = 0
           const float2 y = dev::fma2(make_float2(o[2 * i], o[2 * i + 1]), make_float2(inv, inv), make_float2(0.f, 0.f));
           probe = dev::fma2(y, make_float2(0.f, 0.f), probe);
           v[i] = dev::pack2<T>(y.x, y.y);
@@ -609,7 +612,18 @@ __global__ void __launch_bounds__(384, 1)
         }
       }
       dev::tc_fence_before();  // orders the loads above before the next arrival on p_ready
-      if (__any_sync(0xffffffffu, live && !(probe.x + probe.y == 0.f)) && lane == 0) *bad = 1;
+      const bool odd = live && !(probe.x + probe.y == 0.f);
+      if (__any_sync(0xffffffffu, odd)) {
+        // Rows without a key of any weight are zeros (O may hold 0 times anything). A sum that is NaN is a
+        // score that is NaN or +infinity, of a key that the row sees: so is the row. Others are looked at again.
+        if (odd && l == 0.f)
+          for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
+        const uint32_t again = __ballot_sync(0xffffffffu, odd && l > 0.f);
+        if (lane == 0 && again) {
+          *bad = 1;
+          if (i < kListed) redo[(i * 2 + t) * 4 + quarter] = again;
+        }
+      }
     }
   }
   dev::tc_fence_before();
@@ -620,7 +634,7 @@ __global__ void __launch_bounds__(384, 1)
   }
   if (!*bad) return;
   // Some row met an infinity or NaN, perhaps one that it does not see (weight 0
-  // times the value): rows whose result is not finite are computed again.
+  // times the value): rows whose result is not finite are looked at again.
   Items again(before, listed, a.batch);
   for (int i = 0; again.nth(i) < total; ++i) {
     const Pair p = again.at(a, i);
@@ -628,10 +642,11 @@ __global__ void __launch_bounds__(384, 1)
     for (int t = 0; t < 2; ++t) {
       const Unit u = p.unit(t);
       for (int r = warp; r < u.rows; r += C::kThreads / 32) {
+        if (i < kListed && !(redo[(i * 2 + t) * 4 + (r >> 5)] >> (r & 31) & 1)) continue;
         const T* out = static_cast<const T*>(a.out) + (int64_t)(p.rq.q0 + u.i0 + r) * a.ldo + u.head * D;
         bool wrong = false;
         for (int c = lane; c < D; c += 32) wrong |= !isfinite(dev::to_f32(out[c]));
-        if (__any_sync(0xffffffffu, wrong)) attention_row<T>(a, p.rq, u.i0 + r, u.head, 0, D);
+        if (__any_sync(0xffffffffu, wrong)) attention_row<T, D>(a, p.rq, u.i0 + r, u.head, 0, D);
       }
     }
   }

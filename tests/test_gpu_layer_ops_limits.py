@@ -1,9 +1,12 @@
-"""The layer operators of include/nemo_ops.h at the ends of their ranges."""
+"""The layer operators of include/nemo_ops.h at the ends of their ranges: the smallest and largest values of a type,
+infinities in long prompts, long caches, and launch shapes between those of test_gpu_layer_ops.py."""
+import math
+
 import pytest
 import torch
 
 import layer_ops_ref as ref
-from layer_ops_ref import F32
+from layer_ops_ref import BF16, F16, F32, TORCH
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +37,96 @@ def test_w4_matvec_of_the_smallest_bf16_values(gen, shift, m, n):
     segments = k // group
     slack = (40 + segments / 4) * 2 * ref.U32 * mag + (64 + 4 * segments) * 2.0 ** -150
     ref.close(y, want, ref.U32 * want.abs() + slack)
+
+
+# --- attention_window ------------------------------------------------------------
+
+def milliseconds(call):
+    call()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    call()
+    b.record()
+    torch.cuda.synchronize()
+    return a.elapsed_time(b)
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("q_len", [4, 8192])
+def test_attention_window_one_bad_value_does_not_stall_a_long_call(gen, q_len, bad):
+    """One infinite or NaN element in the first value row, which every query sees: its column is lost, the other
+    columns keep their values, and the call takes a few times as long as on clean values (a warp that walked key by
+    key over every row took several hundred times)."""
+    n, hq, hk, d = 8192, 24, 8, 128
+    q = torch.randn((q_len, hq, d), generator=gen, device="cuda").half()
+    k, v = (torch.randn((n, hk, d), generator=gen, device="cuda").half() for _ in range(2))
+    v[7000] = 0
+    args = (q, k, v, [0, q_len], [0], [n], -1, 0, 0)
+    clean = ref.attention(*args)
+    usual = milliseconds(lambda: ref.attention(*args))
+    v[0, 3, 77] = bad
+    got = ref.attention(*args)
+    took = milliseconds(lambda: ref.attention(*args))
+    lost = torch.zeros((hq, d), dtype=torch.bool, device="cuda")
+    lost[9:12, 77] = True
+    print(f"clean {usual:.3f} ms, with one bad value {took:.3f} ms")
+    assert torch.equal(~torch.isfinite(got), lost.expand_as(got))
+    assert torch.equal(got[:, ~lost], clean[:, ~lost])
+    assert took < 20 * usual
+
+
+@pytest.mark.parametrize("q_len", [4, 8192])
+def test_attention_window_one_bad_key_does_not_stall_a_long_call(gen, q_len):
+    n, hq, hk, d = 8192, 24, 8, 128
+    q = torch.randn((q_len, hq, d), generator=gen, device="cuda").half()
+    k, v = (torch.randn((n, hk, d), generator=gen, device="cuda").half() for _ in range(2))
+    args = (q, k, v, [0, q_len], [0], [n], -1, -1, 0)
+    clean = ref.attention(*args)
+    usual = milliseconds(lambda: ref.attention(*args))
+    k[n - 1, 5, 0] = math.nan
+    got = ref.attention(*args)
+    took = milliseconds(lambda: ref.attention(*args))
+    print(f"clean {usual:.3f} ms, with one bad key {took:.3f} ms")
+    assert torch.isnan(got[:, 15:18]).all()
+    assert torch.equal(got[:, :15], clean[:, :15]) and torch.equal(got[:, 18:], clean[:, 18:])
+    assert took < 20 * usual
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("q_len", [3, 1500])
+def test_attention_window_infinities_and_nan_where_rows_see_them_and_not(gen, dt, q_len):
+    """Bad values of some columns, of either sign, near one another, some of them out of the sight of some queries or
+    of all: each result is what the sum of the visible keys' terms is, and clean columns are those of clean values."""
+    n, hq, hk, d = 1500, 4, 2, 64
+    q = torch.randn((q_len, hq, d), generator=gen, device="cuda").to(TORCH[dt])
+    k, v = (torch.randn((n, hk, d), generator=gen, device="cuda").to(TORCH[dt]) for _ in range(2))
+    left, right, sinks = 60, 3, 2
+    args = (q, k, v, [0, q_len], [0], [n], left, right, sinks)
+    clean = ref.attention(*args)
+    for j, h, c, x in ((0, 0, 1, math.inf), (1, 0, 2, math.nan), (5, 0, 3, math.inf), (700, 1, 4, -math.inf),
+                       (700, 1, 5, math.nan), (703, 1, 4, math.inf), (710, 1, 6, math.inf), (1498, 0, 63, -math.inf),
+                       (1499, 1, 62, math.nan), (1497, 1, slice(None), math.inf)):
+        v[j, h, c] = x
+    got = ref.attention(*args)
+    ok = ref.seen(q_len, n, left, right, sinks).double()
+    for h in range(hq):
+        # counts of the +infinite, -infinite and NaN terms that each result has
+        up, down, nan = (ok @ (f(v[:, h // 2])).double() for f in (torch.isposinf, torch.isneginf, torch.isnan))
+        want = torch.where(nan + up * down > 0, math.nan, torch.where(up > 0, math.inf, -math.inf))
+        want = torch.where(nan + up + down > 0, want, 0.0).to(got.dtype)
+        have = torch.where(torch.isfinite(got[:, h]), 0, got[:, h])
+        assert torch.equal(torch.nan_to_num(have, nan=7.0), torch.nan_to_num(want, nan=7.0))
+        fine = torch.isfinite(got[:, h])
+        ref.close(got[:, h][fine], clean[:, h][fine].double(), 4 * ref.HALF[dt] * 5)
+
+
+@pytest.mark.parametrize("q_len,heads", [(1, 2), (200, 2), (1200, 8)])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_attention_window_rows_without_any_weight_are_zeros_over_bad_values(gen, q_len, heads, bad):
+    n, d = 1200, 64
+    q = torch.rand((q_len, heads, d), generator=gen, device="cuda").half() + 0.5
+    k = torch.full((n, 1, d), -math.inf, dtype=torch.float16, device="cuda")
+    v = torch.randn((n, 1, d), generator=gen, device="cuda").half()
+    v[::7, :, 3] = bad
+    got = ref.attention(q, k, v, [0, q_len], [0], [n], 300, 0, 2)
+    assert (got == 0).all()
