@@ -286,12 +286,15 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
     } else {
       const float inv = 1.f / sum;
       acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-      // (a sum that is not finite is a score that is not: the row is NaN)
-      if (isfinite(sum) && !isfinite(acc.x + acc.y + acc.z + acc.w)) atomicOr(bad, 1u << row);
+    }
+    // A mean of finite values is no larger than they are; the rounded weights' product may be, by half a step.
+    uint2 y = make_uint2(dev::pack2_finite<T>(acc.x, acc.y), dev::pack2_finite<T>(acc.z, acc.w));
+    if (!isfinite(acc.x + acc.y + acc.z + acc.w)) {
+      y = make_uint2(dev::pack2<T>(acc.x, acc.y), dev::pack2<T>(acc.z, acc.w));
+      if (isfinite(sum)) atomicOr(bad, 1u << row);  // (otherwise a score is not: the row is NaN)
     }
     const int qi = global_row / group, head = kvh * group + global_row % group;
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(rq.q0 + qi) * a.ldo + head * D + d0 + c) =
-        make_uint2(dev::pack2<T>(acc.x, acc.y), dev::pack2<T>(acc.z, acc.w));
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(rq.q0 + qi) * a.ldo + head * D + d0 + c) = y;
   }
   __syncthreads();
   uint32_t rest = *bad;

@@ -604,26 +604,42 @@ __global__ void __launch_bounds__(384, 1)
         for (int i = 0; i < 16; ++i) {
           const float2 y = dev::fma2(make_float2(o[2 * i], o[2 * i + 1]), make_float2(inv, inv), make_float2(0.f, 0.f));
           probe = dev::fma2(y, make_float2(0.f, 0.f), probe);
-          v[i] = dev::pack2<T>(y.x, y.y);
+          // (a mean of finite values is no larger than they are; the rounded weights' product may be, by half a step)
+          v[i] = dev::pack2_finite<T>(y.x, y.y);
         }
         if (live) {
           store32(out + c * 32, v);
           store32(out + c * 32 + 16, v + 8);
         }
       }
-      dev::tc_fence_before();  // orders the loads above before the next arrival on p_ready
       const bool odd = live && !(probe.x + probe.y == 0.f);
       if (__any_sync(0xffffffffu, odd)) {
-        // Rows without a key of any weight are zeros (O may hold 0 times anything). A sum that is NaN is a
-        // score that is NaN or +infinity, of a key that the row sees: so is the row. Others are looked at again.
-        if (odd && l == 0.f)
-          for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
+        // Such rows are written with their infinities, and rows without a key of any weight with zeros (O may
+        // hold 0 times anything there). A sum that is NaN is a score that is NaN or +infinity, of a key that the
+        // row sees: so is the row. Others are looked at again.
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          dev::tmem_ld_32x32b_x16(col_o + c, o);
+          dev::tc_wait_ld();
+          if (odd) {
+#pragma unroll
+            for (int k = 0; k < 16; k += 8) {
+              float y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : __uint_as_float(o[k + e]) * inv;
+              *reinterpret_cast<uint4*>(out + c + k) = dev::pack8<T>(y);
+            }
+          }
+          __syncwarp();
+        }
         const uint32_t again = __ballot_sync(0xffffffffu, odd && l > 0.f);
         if (lane == 0 && again) {
           *bad = 1;
           if (i < kListed) redo[(i * 2 + t) * 4 + quarter] = again;
         }
       }
+      dev::tc_fence_before();  // orders the loads above before the next arrival on p_ready
     }
   }
   dev::tc_fence_before();

@@ -123,6 +123,21 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// The same with values past the type's largest one rounded to that, not to infinity.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_finite(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2_finite<__half>(float a, float b) {
+  uint32_t u;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
+  return u;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2_finite<__nv_bfloat16>(float a, float b) {
+  uint32_t u;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
+  return u;
+}
 
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }

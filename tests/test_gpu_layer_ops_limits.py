@@ -130,3 +130,22 @@ def test_attention_window_rows_without_any_weight_are_zeros_over_bad_values(gen,
     v[::7, :, 3] = bad
     got = ref.attention(q, k, v, [0, q_len], [0], [n], 300, 0, 2)
     assert (got == 0).all()
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("q_len,nk,heads", [(1, 300, 1), (1, 5000, 1), (300, 1200, 1), (1200, 1200, 8)])
+def test_attention_window_of_the_largest_values(gen, dt, q_len, nk, heads):
+    """Values at the end of the type: a weighted mean of them is no larger, so it stays finite however the weights
+    round. Here 15 of 16 weights round up by nearly half a step."""
+    d, top = 64, torch.finfo(TORCH[dt]).max
+    q = torch.zeros((q_len, heads, d), dtype=TORCH[dt], device="cuda")
+    k = torch.zeros((nk, heads, d), dtype=TORCH[dt], device="cuda")
+    q[..., 0] = 1
+    k[..., 0] = -1
+    k[::16, :, 0] = 0
+    v = torch.full((nk, heads, d), top, dtype=TORCH[dt], device="cuda")
+    v[..., 1::2] *= -1
+    weight = 0.5 + 0.55 * (2.0 ** -11 if dt == F16 else 2.0 ** -8)  # the type's step there is 2^-11 or 2^-8
+    args = (q, k, v, [0, q_len], [0], [nk], -1, -1, 0)
+    got = ref.attention(*args, scale=-math.log(weight))
+    ref.check_attention(*args, got, scale=-math.log(weight))
