@@ -59,6 +59,22 @@ struct KeyRange {
   }
 };
 
+// Weights are 2^(score - reference), with a reference this far (log2) below the
+// running maximum. f16 has less than 11 bits below 2^-14: beside a weight of 1,
+// the small ones of a long cache would lose them, or all round alike (one key with
+// half of the weight, 131072 with the rest: 3.4e-3 off without, 1.4e-3 with). In
+// the tile kernel more would leave too little room above an old maximum (7: 107 us
+// where 0 and 4 take 103). Where scores are so large that the difference is
+// rounded, it is at most 8.
+template <typename T>
+constexpr float weight_lift() {
+  return 0.f;
+}
+template <>
+constexpr float weight_lift<__half>() {
+  return 4.f;
+}
+
 // Which of 8 elements have an exponent field of ones (an infinity or NaN), and
 // which are NaN: a bit each.
 template <typename T>

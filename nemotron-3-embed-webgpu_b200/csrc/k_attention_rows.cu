@@ -35,8 +35,8 @@ struct RowsCfg {
   // the warps' partial results reuse the ring: [warp][16][D] f32
   static constexpr int kMerge = kWarps * 16 * D * 4;
   static constexpr int kArea = kRing > kMerge ? kRing : kMerge;
-  // behind it: maximum and sum of [warp][16], then what the cluster's blocks send:
-  // of each rank 16 rows of this block's columns, maximum and sum of 16 rows
+  // behind it: reference and sum of [warp][16], then what the cluster's blocks send:
+  // of each rank 16 rows of this block's columns, reference and sum of 16 rows
   static constexpr int kStats = 2 * kWarps * 16 * 4;
   static constexpr int kSent = 16 * D * 4 + 2 * kMaxSplits * 16 * 4;
   static constexpr int kSmem = kArea + kStats + kSent + 64;
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
     }
   }
   const float scale = a.scale * 1.4426950408889634f;  // scores in log2 units
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m: the references of the weights
   float o[D / 8][4];
 #pragma unroll
   for (int n = 0; n < D / 8; ++n)
@@ -161,11 +161,12 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
     float keep[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float mx = m[h];
+      float mx = -INFINITY;
 #pragma unroll
       for (int n = 0; n < kChunk / 8; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      mx = fmaxf(m[h], mx - weight_lift<T>());
       const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen yet: all weights 0
       keep[h] = dev::exp2_approx(m[h] - ref);
       m[h] = mx;
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
   // Every other block of the cluster runs by now, so its shared memory may be written.
   if (splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   // The block's result: a thread has 16 / 4 rows of one column group of four. It
-  // goes to the block that writes these columns (maximum and sum to all).
+  // goes to the block that writes these columns (reference and sum to all).
   constexpr int kQuads = D / 4, kStep = kThreads / kQuads;
   const int quad = threadIdx.x % kQuads, col = quad * 4, owner = col / width;
   const uint32_t to_o = dev::smem_u32(so) + (rank * 16 * width + col - owner * width) * 4;

@@ -8,7 +8,8 @@
 // For each unit and tile of 64 keys:
 //   S = Q . K^T   (tcgen05, f32 in tensor memory)
 //   online softmax by the unit's four warps, one query row per thread
-//   P = 2^(S scale log2 e - m) rounded to the 16-bit type over the columns of S
+//   P = 2^(S scale log2 e - m) rounded to the 16-bit type over the columns of S,
+//   m the running maximum (f16: less weight_lift)
 //   O += P . V    (tcgen05, P from tensor memory, O stays there)
 // Each unit has two S tiles in tensor memory (2 x 64 columns beside 128 of O;
 // two units fill the 512): the products of the next key tile are ready when a
@@ -50,8 +51,8 @@ constexpr int kKeys = 64;           // keys of a tile
 constexpr int kChunks = kKeys / 32;
 constexpr int kMaxRequests = 1024;  // of one launch: their pair counts are summed in shared memory
 constexpr int kListed = 48;         // items of a block that are worked out at its start
-constexpr float kMaxSum = 32768.f;  // sum of a row's weights of one tile against an old maximum, at most
-constexpr float kMaxSlack = 14.f;   // and how far such a maximum may be exceeded (log2): f16 ends at 65504
+constexpr float kMaxSum = 32768.f;  // sum of a row's weights of one tile against an old reference, at most
+constexpr float kMaxSlack = 14.f;   // and how far such a one may be exceeded (log2): f16 ends at 65504
 
 template <int D>
 struct TilesCfg {
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(384, 1)
       // Window tiles [plain0, plain1) whose 64 keys every row of the warp sees.
       const int plain0 = (max(bottom.first - p.lo, 0) + kKeys - 1) / kKeys;
       const int plain1 = max(min(top.last + 1, u.hi) - p.lo, 0) / kKeys;
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f;  // m: the reference of the weights
       int seen = 0;  // tiles of this pair
       for (int j = 0; j < p.tiles; ++j) {
         int base = 0, end = 0;
@@ -492,11 +493,11 @@ __global__ void __launch_bounds__(384, 1)
         for (int c = 0; c < kChunks; ++c)
           dev::tmem_ld_32x32b_x32(col_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
         dev::tc_wait_ld();
-        // A tile that every row sees takes its weights against the running maximum
-        // straight away. They stand if every row's sum is at most 2^15 (with 2^8 as
+        // A tile that every row sees takes its weights against the reference that
+        // it has straight away. They stand if every row's sum is at most 2^15 (with 2^8 as
         // the limit more tiles go twice: 106 us for the 102 above): then no
         // weight is above that either, inside the 16-bit types, and O needs no
-        // rescaling. Otherwise the tile's own maximum is found, the running one
+        // rescaling. Otherwise the tile's own maximum is found, the reference
         // moves and the weights are taken again. (A NaN fails the comparison.)
         if (any == 3 && whole == 3 && seen) {
 #pragma unroll
@@ -528,8 +529,8 @@ __global__ void __launch_bounds__(384, 1)
               for (int k = 0; k < 4; ++k) part[k] = dev::max3(part[k], s[c * 32 + i + 2 * k], s[c * 32 + i + 2 * k + 1]);
           }
           const float tmax = scale * fmaxf(dev::max3(part[0], part[1], part[2]), part[3]);
-          const bool move = __any_sync(0xffffffffu, tmax > m + (whole == 3 ? 0.f : kMaxSlack));
-          const float mnew = move ? fmaxf(m, tmax) : m;
+          const bool move = __any_sync(0xffffffffu, tmax > m + (whole == 3 ? weight_lift<T>() : kMaxSlack));
+          const float mnew = move ? fmaxf(m, tmax - weight_lift<T>()) : m;
           const float neg = mnew == -INFINITY ? 0.f : -mnew;  // no key seen yet: all weights 0
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {

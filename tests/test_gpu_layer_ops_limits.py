@@ -149,3 +149,30 @@ def test_attention_window_of_the_largest_values(gen, dt, q_len, nk, heads):
     args = (q, k, v, [0, q_len], [0], [nk], -1, -1, 0)
     got = ref.attention(*args, scale=-math.log(weight))
     ref.check_attention(*args, got, scale=-math.log(weight))
+
+
+@pytest.mark.parametrize("batch,q_len,nk,heads,warps,share", [
+    (1, 1, 500000, 1, 64, 1.03), (100, 1, 400000, 8, 4, 1.02645), (1, 2048, 131072, 8, 1, 1.03)])
+def test_attention_window_many_small_weights(gen, batch, q_len, nk, heads, warps, share):
+    """Some first keys with half of the weight and a long cache that shares the other half: each small weight keeps
+    the type's relative precision (half a step of f16 for the weights, as much for the result; and each of the
+    nk / warps / 16 instructions of a chain of sums may cut off one f32 step). `warps` of the 16-row kernel share the
+    keys, 16 at a time each, and begin with a large one each."""
+    d = 64
+    q = torch.zeros((batch * q_len, heads, d), dtype=torch.float16, device="cuda")
+    k = torch.zeros((nk, heads, d), dtype=torch.float16, device="cuda")
+    q[..., 0] = 1
+    k[..., 0] = -1
+    v = 1 + torch.rand((nk, heads, d), generator=gen, device="cuda").half()
+    first = range(0, 16 * warps, 16)
+    for j in first:
+        k[j], v[j] = 0, 0
+    args = (q, k, v, [b * q_len for b in range(batch + 1)], [0] * batch, [nk] * batch, -1, -1, 0)
+    scale = math.log(share * nk / len(first))
+    got = ref.attention(*args, scale=scale).double()
+    w = torch.full((nk,), math.exp(-scale), dtype=torch.float64, device="cuda")
+    w[list(first)] = 1
+    want = torch.stack([w @ v[:, h].double() for h in range(heads)]) / w.sum()
+    error = float(((got - want) / want).abs().max())
+    print(f"relative error {error:.2e}")
+    assert error <= 2 * 2.0 ** -11 + 2.0 ** -15 + nk / warps / 16 * 2.0 ** -23
