@@ -224,8 +224,9 @@ int nemo_rope_inv_freq(int scaling, double theta, int rotary_dim, double factor,
  * 16-bit x takes NULL. y is F16, BF16 or F32. Sums are f32 or finer and y is
  * rounded once; 16-bit elements of x below 2^-19 of the largest of their 32 to
  * 128 neighbours may be rounded to 2^-30 of it. An infinity or NaN in a row of
- * x makes its row of y infinite or NaN. m > 16 is refused: nemo_op_qmatmul serves
- * batches. n and k are at most 2^30. d_x and ldx need the alignment of one
+ * x makes its row of y infinite or NaN. m > 16 is refused: more rows take a call
+ * for each 16 of them, which reads the weights each time (no other entry takes
+ * this format). n and k are at most 2^30. d_x and ldx need the alignment of one
  * element only. */
 int nemo_op_w4_matvec(int x_dtype, const void* d_x, int64_t ldx, const void* d_x_scales, int x_group, const void* d_w4,
                       int scale_dtype, const void* d_scales, const void* d_zeros, int group, int m, int n, int k,

@@ -202,7 +202,7 @@ int nemo_op_w4_matvec(int x_dtype, const void* d_x, int64_t ldx, const void* d_x
     if (!is16(x_dtype) && !is8(x_dtype)) return refuse(op, "x must be f16, bf16, e4m3 or i8");
     if (!is16(scale_dtype)) return refuse(op, "scales must be f16 or bf16");
     if (!is16(y_dtype) && y_dtype != kDtF32) return refuse(op, "y must be f16, bf16 or f32");
-    if (m < 0 || m > 16) return refuse(op, "m must be in [0, 16]; nemo_op_qmatmul serves larger batches");
+    if (m < 0 || m > 16) return refuse(op, "m must be in [0, 16]: more rows take a call for each 16 of them");
     if (n < 1 || k < 1 || n > 1 << 30 || k > 1 << 30) return refuse(op, "n and k must be positive and at most 2^30");
     if (group != 32 && group != 64 && group != 128) return refuse(op, "group must be 32, 64 or 128");
     if (k % group) return refuse(op, "group must divide k");

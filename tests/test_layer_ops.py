@@ -139,3 +139,11 @@ def test_inv_freq_refuses(args):
     assert L.nemo_rope_inv_freq(*args, out.ctypes.data_as(ctypes.c_void_p), ctypes.byref(mag)) == ERR_ARGS
     assert L.nemo_last_error().startswith(b"nemo_rope_inv_freq")
     assert L.nemo_rope_inv_freq(0, 1e4, 64, 1.0, 1.0, 1.0, 2.0, None, ctypes.byref(mag)) == ERR_ARGS
+
+
+def test_w4_matvec_sends_larger_batches_to_no_entry_of_other_formats():
+    """nemo_op_qmatmul takes Q4_K, Q6_K, Q4_0 and tile32 weights and f16 x, none of these."""
+    L = load_library()
+    assert L.nemo_op_w4_matvec(*dict(W4, m=17).values()) == ERR_ARGS
+    text = L.nemo_last_error().decode()
+    assert "qmatmul" not in text and "each 16" in text
