@@ -136,6 +136,7 @@ int nemo_rope_inv_freq(int scaling, double theta, int rotary_dim, double factor,
     const int half = rotary_dim / 2;
     const double two_pi = 2.0 * M_PI;
     if (scaling == NEMO_ROPE_NTK) theta *= pow(factor, (double)rotary_dim / (rotary_dim - 2));
+    if (isinf(theta)) return refuse(op, "the scaled theta is not finite");
     // the pair that turns `turns` times in the original context
     auto pair_of = [&](double turns) {
       return rotary_dim * log(original_context / (turns * two_pi)) / (2.0 * log(theta));

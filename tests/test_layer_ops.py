@@ -147,3 +147,13 @@ def test_w4_matvec_sends_larger_batches_to_no_entry_of_other_formats():
     assert L.nemo_op_w4_matvec(*dict(W4, m=17).values()) == ERR_ARGS
     text = L.nemo_last_error().decode()
     assert "qmatmul" not in text and "each 16" in text
+
+
+@pytest.mark.parametrize("theta,rotary,factor", [(1e300, 64, 1e10), (1e4, 4, 1e200)])
+def test_inv_freq_refuses_a_scaled_base_that_overflows(theta, rotary, factor):
+    """theta * factor^(r / (r - 2)) past the largest double: every frequency but the first would be 0."""
+    out, mag = np.zeros(64), ctypes.c_float()
+    L = load_library()
+    assert L.nemo_rope_inv_freq(2, theta, rotary, factor, 0.0, 0.0, 0.0, out.ctypes.data_as(ctypes.c_void_p),
+                                ctypes.byref(mag)) == ERR_ARGS
+    assert b"scaled" in L.nemo_last_error()
