@@ -260,6 +260,14 @@ int nemo_op_attention_window(int dtype, const void* d_q, int64_t ldq, const void
                              int max_k, int left, int right, int sinks, float scale, void* d_out, int64_t ldo,
                              void* d_err, void* stream);
 
+/* On the host, how nemo_op_attention_window runs a call of these sizes on a
+ * device of `sms` SMs that can place clusters of max_cluster blocks (16 on a
+ * whole B200): *tiles 1 on 128-query tensor-core tiles, 0 on 16-row ones, whose
+ * keys *splits blocks of a cluster share. */
+int nemo_op_attention_window_form(int q_heads, int kv_heads, int head_dim, int batch, int q_rows, int k_rows, int max_q,
+                                  int max_k, int left, int right, int sinks, int sms, int max_cluster, int* tiles,
+                                  int* splits);
+
 /* Routing of the head-parallel path (no reference counterpart; the index
  * functions its QKV GEMM and attention epilogues use, exported for layout
  * tests without a GPU), n_devices in {2, 4, 8}:

@@ -306,24 +306,56 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_c
   }
 }
 
+// 16-row tiles of a request and kv head.
+int64_t row_tiles(const AttnWindowArgs& a) { return ((int64_t)a.max_q * (a.q_heads / a.kv_heads) + 15) / 16; }
+
+// Largest cluster of the kernel that the current device can place: 16 blocks are
+// more than is portable, and a partition of a GPU may have no room for them.
+template <typename K>
+cudaError_t largest_cluster(K* kernel, size_t smem, int* blocks) {
+  for (*blocks = kMaxSplits; *blocks > 1; *blocks /= 2) {
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = *blocks, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(*blocks), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr, cfg.numAttrs = 1;
+    int clusters = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+    if (e == cudaSuccess && clusters > 0) break;
+    if (e != cudaSuccess && e != cudaErrorInvalidClusterSize) return e;
+    cudaGetLastError();
+  }
+  return cudaSuccess;
+}
+
 template <typename T, int D>
 cudaError_t launch_rows(const AttnWindowArgs& a, cudaStream_t s) {
   constexpr int kStages = 3;
   using C = RowsCfg<D, kStages>;
   auto kernel = attention_rows_kernel<T, D, kStages>;
-  static bool configured[64] = {};
+  static int max_splits[64] = {};  // 0: the kernel is not set up on that device yet
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64) return cudaErrorInvalidDevice;
-  if (!configured[dev]) {
+  if (!max_splits[dev]) {
+    int blocks = 1;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = largest_cluster(kernel, C::kSmem, &blocks);
     if (e != cudaSuccess) return e;
-    configured[dev] = true;
+    max_splits[dev] = blocks;
   }
-  const int group = a.q_heads / a.kv_heads;
-  const int64_t tiles = ((int64_t)a.max_q * group + 15) / 16;
+  const int64_t tiles = row_tiles(a);
+  const int splits = attention_splits(a, max_splits[dev]);
+  const dim3 grid((unsigned)(tiles * splits), a.kv_heads, a.batch);
+  return launch_overlapped(kernel, grid, dim3(kThreads), C::kSmem, s, dim3(splits, 1), a, splits, (int)tiles);
+}
+
+}  // namespace
+
+int attention_splits(const AttnWindowArgs& a, int max_splits) {
   const int64_t keys = visible_keys(a, 16);
   const int64_t chunks = (keys + kChunk - 1) / kChunk;
   // Split the keys over a cluster while two blocks an SM are not reached and
@@ -331,15 +363,13 @@ cudaError_t launch_rows(const AttnWindowArgs& a, cudaStream_t s) {
   // a tile, 24.9 with one); beyond that, up to eight, while it keeps 32, which
   // levels ragged lengths (16 tokens on up to 32768 keys: 193 us, 256 without).
   int splits = 1;
-  const int64_t blocks = tiles * a.kv_heads * a.batch;
-  while (splits < kMaxSplits && chunks >= splits * 2 * kWarps * 2 &&
-         (blocks * splits * 2 <= 296 || (blocks * splits * 2 <= 8 * 148 && chunks >= splits * 2 * kWarps * 32)))
+  const int64_t blocks = row_tiles(a) * a.kv_heads * a.batch, sms = a.sms;
+  if (max_splits > kMaxSplits) max_splits = kMaxSplits;
+  while (splits * 2 <= max_splits && chunks >= splits * 2 * kWarps * 2 &&
+         (blocks * splits * 2 <= 2 * sms || (blocks * splits * 2 <= 8 * sms && chunks >= splits * 2 * kWarps * 32)))
     splits *= 2;
-  const dim3 grid((unsigned)(tiles * splits), a.kv_heads, a.batch);
-  return launch_overlapped(kernel, grid, dim3(kThreads), C::kSmem, s, dim3(splits, 1), a, splits, (int)tiles);
+  return splits;
 }
-
-}  // namespace
 
 cudaError_t launch_attention_rows(const AttnWindowArgs& a, cudaStream_t s) {
   if (a.head_dim == 64)

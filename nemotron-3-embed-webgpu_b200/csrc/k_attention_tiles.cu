@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(384, 1)
 }  // namespace
 
 template <typename T, int D>
-static cudaError_t launch_tiles(AttnWindowArgs a, int sms, cudaStream_t s) {
+static cudaError_t launch_tiles(AttnWindowArgs a, cudaStream_t s) {
   using C = TilesCfg<D>;
   auto kernel = attention_tiles_kernel<T, D>;
   static bool configured[64] = {};
@@ -696,7 +696,7 @@ static cudaError_t launch_tiles(AttnWindowArgs a, int sms, cudaStream_t s) {
   for (int b = 0; b < batch; b += kMaxRequests) {
     a.batch = batch - b < kMaxRequests ? batch - b : kMaxRequests;
     const int64_t items = pairs * a.batch;
-    e = launch_overlapped(kernel, dim3((unsigned)(items < sms ? items : sms)), dim3(C::kThreads), C::kSmem, s,
+    e = launch_overlapped(kernel, dim3((unsigned)(items < a.sms ? items : a.sms)), dim3(C::kThreads), C::kSmem, s,
                           dim3(1, 1), mq, mk, mv, a);
     if (e != cudaSuccess) return e;
     a.q_off += kMaxRequests, a.k_start += kMaxRequests, a.k_len += kMaxRequests;
@@ -720,20 +720,20 @@ int64_t visible_keys(const AttnWindowArgs& a, int rows) {
 // 5 + 0.85 a step of 64 keys and round of pairs over the SMs. 16 x 8 queries on
 // 1500 keys 31 against 51, 16 x 32 88 against 51; 1 x 64 on 16384 111 against
 // 222, 1 x 128 204 against 224.
-cudaError_t launch_attention_window(const AttnWindowArgs& a, cudaStream_t s) {
-  int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return e;
+bool attention_on_tiles(const AttnWindowArgs& a) {
   const int group = a.q_heads / a.kv_heads;
   const double row_tiles = (double)(((int64_t)a.max_q * group + 15) / 16) * a.kv_heads * a.batch;
   const double pairs = (double)((((int64_t)a.max_q + kRows - 1) / kRows * group + 1) / 2) * a.kv_heads * a.batch;
   const double few = 6 + row_tiles * visible_keys(a, 16) / 13000;
-  const double many = 5 + ceil(pairs / sms) * visible_keys(a, kRows + kKeys) * (0.85 / kKeys);
-  if (few <= many || a.k_rows == 0) return launch_attention_rows(a, s);
+  const double many = 5 + ceil(pairs / a.sms) * visible_keys(a, kRows + kKeys) * (0.85 / kKeys);
+  return few > many && a.k_rows > 0;
+}
+
+cudaError_t launch_attention_window(const AttnWindowArgs& a, cudaStream_t s) {
+  if (!attention_on_tiles(a)) return launch_attention_rows(a, s);
   if (a.head_dim == 64)
-    return a.dtype == kDtBF16 ? launch_tiles<__nv_bfloat16, 64>(a, sms, s) : launch_tiles<__half, 64>(a, sms, s);
-  return a.dtype == kDtBF16 ? launch_tiles<__nv_bfloat16, 128>(a, sms, s) : launch_tiles<__half, 128>(a, sms, s);
+    return a.dtype == kDtBF16 ? launch_tiles<__nv_bfloat16, 64>(a, s) : launch_tiles<__half, 64>(a, s);
+  return a.dtype == kDtBF16 ? launch_tiles<__nv_bfloat16, 128>(a, s) : launch_tiles<__half, 128>(a, s);
 }
 
 }  // namespace nemo

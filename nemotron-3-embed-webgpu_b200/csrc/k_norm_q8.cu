@@ -222,7 +222,7 @@ cudaError_t launch_rmsnorm_q8(const NormQ8Args& a, cudaStream_t s) {
   // one), and four where the grid is many waves and fewer instructions count
   // (24000 rows: 58 us with four, 61 with two, 84 with one).
   const int64_t total = (int64_t)a.rows * vectors;
-  int nv = total <= 148 * 256 ? 1 : vectors <= 128 ? (vectors <= 32 ? 1 : vectors <= 64 ? 2 : 4) : total < 4000000 ? 2 : 4;
+  int nv = total <= a.sms * 256 ? 1 : vectors <= 128 ? (vectors <= 32 ? 1 : vectors <= 64 ? 2 : 4) : total < 4000000 ? 2 : 4;
   while (vectors > nv * (nv == 4 ? 1024 : 512)) nv *= 2;
   const int wpr = (vectors + 32 * nv - 1) / (32 * nv);
   const int rows_per_block = wpr >= 4 ? 1 : 4 / wpr;

@@ -153,7 +153,7 @@ cudaError_t launch_rope_apply(const RopeApplyArgs& a, cudaStream_t s) {
   }
   const int heads = a.q_heads + a.k_heads;
   // few tokens: more threads each (one token 1.8 us with 256, 2.5 with 128)
-  const int threads = a.tokens <= 8 * 148 ? 256 : 128;
+  const int threads = a.tokens <= 8 * a.sms ? 256 : 128;
   int rows = items >= threads ? 1 : threads / items;
   if (rows > heads) rows = heads;
   const dim3 block(items, rows);

@@ -808,7 +808,7 @@ cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s) {
       p.stages = smem_of(r, 3) <= kSmemLimit / 2 ? 3 : 2;
       const size_t bytes = smem_of(r, p.stages);
       if (bytes > kSmemLimit) continue;
-      const int resident = (bytes <= kSmemLimit / 2 ? 2 : 1) * 148 / p.splits;
+      const int resident = (bytes <= kSmemLimit / 2 ? 2 : 1) * a.sms / p.splits;
       for (p.wk = 1; p.wk <= 8; p.wk *= 2) {
         const int64_t block_rows = 16LL * r * (8 / p.wk), tiles = (a.n + block_rows - 1) / block_rows;
         p.slice_segs = (p.panel_segs + p.wk - 1) / p.wk;

@@ -47,14 +47,16 @@ class BufferDevice {
       NEMO_CUDA_TRY(cudaSetDevice(device));
       switched_ = true;
     }
+    NEMO_CUDA_TRY(cudaDeviceGetAttribute(&sms_, cudaDevAttrMultiProcessorCount, device >= 0 ? device : before_));
     return kOk;
   }
+  int sms() const { return sms_; }  // of the device
   ~BufferDevice() {
     if (switched_) cudaSetDevice(before_);
   }
 
  private:
-  int before_ = 0;
+  int before_ = 0, sms_ = 0;
   bool switched_ = false;
 };
 
@@ -114,7 +116,7 @@ int nemo_op_rmsnorm_q8(int dtype, const void* d_x, int64_t ldx, const void* d_re
     a.scales = (float*)d_scales;
     a.ldx = ldx, a.ldr = ldr, a.lds = lds, a.ldq = ldq;
     a.rows = rows, a.width = width, a.group = group, a.groups = group ? (width + group - 1) / group : 1;
-    a.eps = eps, a.dtype = dtype, a.out_dtype = out_dtype;
+    a.eps = eps, a.dtype = dtype, a.out_dtype = out_dtype, a.sms = device.sms();
     return launched(op, launch_rmsnorm_q8(a, (cudaStream_t)stream));
   });
 }
@@ -190,7 +192,7 @@ int nemo_op_rope_apply(int dtype, int layout, const void* d_q, int64_t ldq, int 
     a.inv_freq = (const double*)d_inv_freq, a.positions = (const int*)d_positions;
     a.ldq = ldq, a.ldk = ldk, a.ldqo = ldqo, a.ldko = ldko;
     a.q_heads = q_heads, a.k_heads = k_heads, a.head_dim = head_dim, a.rotary_dim = rotary_dim, a.tokens = tokens;
-    a.magnitude = magnitude, a.dtype = dtype, a.layout = layout;
+    a.magnitude = magnitude, a.dtype = dtype, a.layout = layout, a.sms = device.sms();
     return launched(op, launch_rope_apply(a, (cudaStream_t)stream));
   });
 }
@@ -223,7 +225,7 @@ int nemo_op_w4_matvec(int x_dtype, const void* d_x, int64_t ldx, const void* d_x
     a.x = d_x, a.x_scales = (const float*)d_x_scales, a.w = (const uint8_t*)d_w4;
     a.scales = (const uint16_t*)d_scales, a.zeros = (const uint8_t*)d_zeros, a.y = d_y;
     a.ldx = ldx, a.ldy = ldy, a.x_dtype = x_dtype, a.scale_dtype = scale_dtype, a.y_dtype = y_dtype;
-    a.x_group = x_group, a.group = group, a.m = m, a.n = n, a.k = k;
+    a.x_group = x_group, a.group = group, a.m = m, a.n = n, a.k = k, a.sms = device.sms();
     return launched(op, launch_w4_matvec(a, (cudaStream_t)stream));
   });
 }
@@ -267,8 +269,27 @@ int nemo_op_attention_window(int dtype, const void* d_q, int64_t ldq, const void
     a.q_heads = q_heads, a.kv_heads = kv_heads, a.head_dim = head_dim, a.batch = batch;
     a.q_rows = q_rows, a.k_rows = k_rows, a.max_q = max_q < q_rows ? max_q : q_rows;
     a.max_k = max_k < k_rows ? max_k : k_rows;
-    a.left = left, a.right = right, a.sinks = sinks, a.scale = scale, a.dtype = dtype;
+    a.left = left, a.right = right, a.sinks = sinks, a.scale = scale, a.dtype = dtype, a.sms = device.sms();
     return launched(op, launch_attention_window(a, (cudaStream_t)stream));
+  });
+}
+
+int nemo_op_attention_window_form(int q_heads, int kv_heads, int head_dim, int batch, int q_rows, int k_rows, int max_q,
+                                  int max_k, int left, int right, int sinks, int sms, int max_cluster, int* tiles,
+                                  int* splits) {
+  const char* op = "nemo_op_attention_window_form";
+  return guarded(op, [&]() -> int {
+    if (kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || batch < 1 || q_rows < 1 || k_rows < 0 || max_q < 1 ||
+        max_k < 0 || left < -1 || right < -1 || sinks < 0 || sms < 1 || max_cluster < 1)
+      return refuse(op, "sizes out of range");
+    if (!tiles || !splits) return refuse(op, "null buffer");
+    AttnWindowArgs a = {};
+    a.q_heads = q_heads, a.kv_heads = kv_heads, a.head_dim = head_dim, a.batch = batch, a.q_rows = q_rows;
+    a.k_rows = k_rows, a.max_q = max_q < q_rows ? max_q : q_rows, a.max_k = max_k < k_rows ? max_k : k_rows;
+    a.left = left, a.right = right, a.sinks = sinks, a.sms = sms;
+    *tiles = attention_on_tiles(a);
+    *splits = *tiles ? 1 : attention_splits(a, max_cluster);
+    return kOk;
   });
 }
 

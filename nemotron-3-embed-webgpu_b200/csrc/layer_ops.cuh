@@ -23,6 +23,7 @@ struct NormQ8Args {
   int rows, width, group, groups;
   float eps;
   int dtype, out_dtype;
+  int sms;  // of the device
 };
 cudaError_t launch_rmsnorm_q8(const NormQ8Args& a, cudaStream_t s);
 
@@ -37,6 +38,7 @@ struct RopeApplyArgs {
   int q_heads, k_heads, head_dim, rotary_dim, tokens;
   float magnitude;
   int dtype, layout;
+  int sms;
 };
 cudaError_t launch_rope_apply(const RopeApplyArgs& a, cudaStream_t s);
 
@@ -50,6 +52,7 @@ struct W4Args {
   int64_t ldx, ldy;
   int x_dtype, scale_dtype, y_dtype;
   int x_group, group, m, n, k;
+  int sms;
 };
 cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s);
 
@@ -67,8 +70,13 @@ struct AttnWindowArgs {
   int left, right, sinks;  // left, right < 0: unbounded
   float scale;
   int dtype;
+  int sms;
 };
 cudaError_t launch_attention_window(const AttnWindowArgs& a, cudaStream_t s);
+// Whether a call runs on the 128-query tiles; otherwise blocks that share the
+// keys of a 16-row tile, of at most max_splits in a cluster.
+bool attention_on_tiles(const AttnWindowArgs& a);
+int attention_splits(const AttnWindowArgs& a, int max_splits);
 
 // Launches with programmatic dependent launch: the grid may start while the
 // previous kernel of the stream drains, which hides the launch latency. Every

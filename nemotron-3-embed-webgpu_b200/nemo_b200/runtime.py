@@ -97,6 +97,7 @@ def load_library() -> ctypes.CDLL:
         "nemo_op_w4_matvec": (I, [I, P, I64, P, I, P, I, P, P, I, I, I, I, I, P, I64, P]),
         "nemo_op_attention_window": (I, [I, P, I64, P, I64, P, I64, I, I, I, P, P, P, I, I, I, I, I, I, I, I, F32, P,
                                          I64, P, P]),
+        "nemo_op_attention_window_form": (I, [I, I, I, I, I, I, I, I, I, I, I, I, I, P, P]),
         "nemo_hp_qkv_route": (I, [I, P, P, P]),
         "nemo_hp_row_owner": (I, [I, I, I, P]),
         "nemo_tokenizer_load": (I, [P, S, ctypes.POINTER(P)]),

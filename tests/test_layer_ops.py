@@ -157,3 +157,34 @@ def test_inv_freq_refuses_a_scaled_base_that_overflows(theta, rotary, factor):
     assert L.nemo_rope_inv_freq(2, theta, rotary, factor, 0.0, 0.0, 0.0, out.ctypes.data_as(ctypes.c_void_p),
                                 ctypes.byref(mag)) == ERR_ARGS
     assert b"scaled" in L.nemo_last_error()
+
+
+def window_form(q_heads=24, kv_heads=8, head_dim=128, batch=1, q_rows=1, k_rows=8192, max_q=1, max_k=8192, left=-1,
+                right=0, sinks=0, sms=148, max_cluster=16):
+    tiles, splits = ctypes.c_int(), ctypes.c_int()
+    rc = load_library().nemo_op_attention_window_form(q_heads, kv_heads, head_dim, batch, q_rows, k_rows, max_q, max_k,
+                                                      left, right, sinks, sms, max_cluster, ctypes.byref(tiles),
+                                                      ctypes.byref(splits))
+    assert rc == 0, load_library().nemo_last_error()
+    return tiles.value, splits.value
+
+
+def test_attention_window_forms():
+    """Few queries on 16-row tiles whose keys up to 16 blocks share, prompts on 128-query ones."""
+    assert window_form() == (0, 16)
+    assert window_form(max_k=100) == (0, 1)
+    assert window_form(batch=16, q_rows=16, max_k=32768, k_rows=16 * 32768) == (0, 8)
+    assert window_form(q_rows=8192, max_q=8192)[0] == 1
+    assert window_form(q_rows=8192, max_q=8192, k_rows=0, max_k=0)[0] == 0
+
+
+def test_attention_window_splits_fit_the_device():
+    """A device that cannot place a cluster of 16, or with few SMs, gets fewer blocks a tile."""
+    for cluster in (1, 2, 4, 8, 16):
+        assert window_form(max_cluster=cluster) == (0, cluster)
+    assert window_form(max_cluster=11) == (0, 8)
+    # one tile a kv head: 8 blocks, as many again for each doubling up to two an SM, then 8 an SM of long keys
+    assert window_form(max_k=1024, sms=8) == (0, 2)
+    assert window_form(max_k=32768, k_rows=32768, sms=8) == (0, 8)
+    L = load_library()
+    assert L.nemo_op_attention_window_form(3, 2, 128, 1, 1, 1, 1, 1, -1, -1, 0, 148, 16, None, None) == ERR_ARGS
