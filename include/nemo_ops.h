@@ -232,6 +232,13 @@ int nemo_op_w4_matvec(int x_dtype, const void* d_x, int64_t ldx, const void* d_x
                       int scale_dtype, const void* d_scales, const void* d_zeros, int group, int m, int n, int k,
                       int y_dtype, void* d_y, int64_t ldy, void* stream);
 
+/* On the host, how nemo_op_w4_matvec runs a call of these sizes on a device of
+ * `sms` SMs: *digits 1 if x goes as 8-bit digits, 0 as 16-bit products; *rows
+ * weight rows and one of *slices column slices a warp; rows of x in *panels;
+ * *blocks blocks of *shared_bytes. (x_group is read for 8-bit x only.) */
+int nemo_op_w4_matvec_form(int x_dtype, int x_group, int group, int m, int n, int k, int sms, int* digits, int* rows,
+                           int* slices, int* panels, int* blocks, int* shared_bytes);
+
 /* Grouped-query attention with a sliding window and first tokens that stay
  * visible, for prompts, whole documents and single tokens against a cache.
  * Request b has the query rows d_q_off[b] .. d_q_off[b + 1] - 1 (int32

@@ -56,7 +56,8 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr size_t kSmemLimit = 227 * 1024;
+constexpr size_t kSmemLimit = 227 * 1024;           // of a block
+constexpr size_t kSmemOfTwo = (228 / 2 - 1) * 1024;  // of each of two blocks an SM, which keeps 1 KB for a block
 
 constexpr int kChunk = 256;   // columns of a copy
 constexpr int kPitch = kChunk / 2;
@@ -72,6 +73,9 @@ struct W4Plan {
   int tiles;       // block tiles (8 / wk x 16 R rows)
   int blocks;      // blocks over the tiles
   int stages;      // chunks in flight
+  int tile_rows;   // R: 16-row tiles of a warp
+  bool digits;     // the form
+  size_t smem;
   int cols;        // columns of x's operand in shared memory: m rounded up to 1, 2, 4, 8 or 16, or m's digits
   int off_x, off_xs, off_zero, off_red;  // byte offsets in shared memory (the warps' stages at 0)
 };
@@ -754,14 +758,12 @@ cudaError_t launch_seg(const W4Plan& p, int seg, int r, bool xg, size_t smem, cu
 
 }  // namespace
 
-cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s) {
-  const bool xg = a.x_scales && a.x_group < a.k;
-  const int seg = xg && a.x_group < a.group ? a.x_group : a.group;
-  W4Plan best = {};
+namespace {
+
+// The plan of a call whose x has scales per group if xg. False if none fits.
+bool plan_w4(const W4Args& a, bool xg, int seg, W4Plan& best) {
   double best_cost = 0;
-  size_t best_smem = 0;
-  int best_r = 0;
-  bool best_digits = false;
+  best.tile_rows = 0;
   // Digits or floating point, 16 or 32 rows a warp, slices of a panel: whatever
   // has the least modelled time. That is the rounds of blocks over the SMs,
   // times the chunks of a slice (1 with 32 rows, 0.6 with 16; digits cost less
@@ -805,10 +807,10 @@ cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s) {
     const double prepare = digits ? (double)a.m * panel_k / 8 / kThreads * (a.x_dtype == kDtI8 ? 0.04 : 0.15) : 0;
     for (int r = 1; r <= 2; ++r) {
       // three stages where two blocks still fit an SM, or two
-      p.stages = smem_of(r, 3) <= kSmemLimit / 2 ? 3 : 2;
+      p.stages = smem_of(r, 3) <= kSmemOfTwo ? 3 : 2;
       const size_t bytes = smem_of(r, p.stages);
       if (bytes > kSmemLimit) continue;
-      const int resident = (bytes <= kSmemLimit / 2 ? 2 : 1) * a.sms / p.splits;
+      const int resident = (bytes <= kSmemOfTwo ? 2 : 1) * a.sms / p.splits;
       for (p.wk = 1; p.wk <= 8; p.wk *= 2) {
         const int64_t block_rows = 16LL * r * (8 / p.wk), tiles = (a.n + block_rows - 1) / block_rows;
         p.slice_segs = (p.panel_segs + p.wk - 1) / p.wk;
@@ -816,17 +818,43 @@ cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s) {
         const double cost = (double)((tiles + resident - 1) / resident) *
                                 (chunks * (r == 1 ? 0.6 : 1.0) * (digits ? digit_chunk : 1.0) + (p.splits > 1 ? 2.0 : 0.35)) +
                             prepare;
-        if (best_r && cost >= best_cost) continue;
+        if (best.tile_rows && cost >= best_cost) continue;
         p.tiles = (int)tiles;
         p.blocks = p.tiles < resident ? p.tiles : resident;
-        best = p, best_cost = cost, best_smem = bytes, best_r = r, best_digits = digits;
+        p.tile_rows = r, p.digits = digits, p.smem = bytes;
+        best = p, best_cost = cost;
       }
     }
   }
-  if (!best_r) return cudaErrorInvalidValue;
-  if (best_digits) return launch_seg<int8_t>(best, seg, best_r, xg, best_smem, s);
-  return a.x_dtype == kDtBF16 ? launch_seg<__nv_bfloat16>(best, seg, best_r, xg, best_smem, s)
-                              : launch_seg<__half>(best, seg, best_r, xg, best_smem, s);
+  return best.tile_rows > 0;
+}
+
+// Columns of a segment, and whether x has a scale for each of its groups.
+int w4_segment(const W4Args& a, bool x_scales, bool& xg) {
+  xg = x_scales && a.x_group < a.k;
+  return xg && a.x_group < a.group ? a.x_group : a.group;
+}
+
+}  // namespace
+
+bool w4_form(const W4Args& a, bool x_scales, W4Form& form) {
+  bool xg;
+  const int seg = w4_segment(a, x_scales, xg);
+  W4Plan p;
+  if (!plan_w4(a, xg, seg, p)) return false;
+  form.digits = p.digits, form.rows = 16 * p.tile_rows, form.slices = p.wk, form.panels = p.panels;
+  form.cluster = p.splits, form.smem = p.smem, form.blocks = p.blocks * p.splits;
+  return true;
+}
+
+cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s) {
+  bool xg;
+  const int seg = w4_segment(a, a.x_scales != nullptr, xg);
+  W4Plan p;
+  if (!plan_w4(a, xg, seg, p)) return cudaErrorInvalidValue;
+  if (p.digits) return launch_seg<int8_t>(p, seg, p.tile_rows, xg, p.smem, s);
+  return a.x_dtype == kDtBF16 ? launch_seg<__nv_bfloat16>(p, seg, p.tile_rows, xg, p.smem, s)
+                              : launch_seg<__half>(p, seg, p.tile_rows, xg, p.smem, s);
 }
 
 }  // namespace nemo

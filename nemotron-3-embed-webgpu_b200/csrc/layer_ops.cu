@@ -230,6 +230,25 @@ int nemo_op_w4_matvec(int x_dtype, const void* d_x, int64_t ldx, const void* d_x
   });
 }
 
+int nemo_op_w4_matvec_form(int x_dtype, int x_group, int group, int m, int n, int k, int sms, int* digits, int* rows,
+                           int* slices, int* panels, int* blocks, int* shared_bytes) {
+  const char* op = "nemo_op_w4_matvec_form";
+  return guarded(op, [&]() -> int {
+    if ((!is16(x_dtype) && !is8(x_dtype)) || m < 1 || m > 16 || n < 1 || k < 1 || n > 1 << 30 || k > 1 << 30 ||
+        (group != 32 && group != 64 && group != 128) || k % group || sms < 1 ||
+        (is8(x_dtype) && x_group != 32 && x_group != 64 && x_group != 128 && x_group < k))
+      return refuse(op, "sizes or types out of range");
+    if (!digits || !rows || !slices || !panels || !blocks || !shared_bytes) return refuse(op, "null buffer");
+    W4Args a = {};
+    a.x_dtype = x_dtype, a.x_group = x_group, a.group = group, a.m = m, a.n = n, a.k = k, a.sms = sms;
+    W4Form f;
+    if (!w4_form(a, is8(x_dtype), f)) return refuse(op, "no form fits");
+    *digits = f.digits, *rows = f.rows, *slices = f.slices, *panels = f.panels, *blocks = f.blocks;
+    *shared_bytes = (int)f.smem;
+    return kOk;
+  });
+}
+
 int nemo_op_attention_window(int dtype, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v,
                              int64_t ldv, int q_heads, int kv_heads, int head_dim, const void* d_q_off,
                              const void* d_k_start, const void* d_k_len, int batch, int q_rows, int k_rows, int max_q,

@@ -55,6 +55,15 @@ struct W4Args {
   int sms;
 };
 cudaError_t launch_w4_matvec(const W4Args& a, cudaStream_t s);
+// How a call runs (sizes, types and SMs of `a`; x with scales or not).
+struct W4Form {
+  bool digits;     // x as 8-bit digits, otherwise 16-bit products
+  int rows;        // weight rows of a warp
+  int slices;      // of a panel, a warp each
+  int panels, cluster, blocks;
+  size_t smem;     // of a block
+};
+bool w4_form(const W4Args& a, bool x_scales, W4Form& form);
 
 struct AttnWindowArgs {
   const void* q;

@@ -95,6 +95,7 @@ def load_library() -> ctypes.CDLL:
         "nemo_op_rope_apply": (I, [I, I, P, I64, I, P, I64, I, I, I, P, F32, P, I, P, I64, P, I64, P]),
         "nemo_rope_inv_freq": (I, [I, F64, I, F64, F64, F64, F64, P, ctypes.POINTER(F32)]),
         "nemo_op_w4_matvec": (I, [I, P, I64, P, I, P, I, P, P, I, I, I, I, I, P, I64, P]),
+        "nemo_op_w4_matvec_form": (I, [I, I, I, I, I, I, I, P, P, P, P, P, P]),
         "nemo_op_attention_window": (I, [I, P, I64, P, I64, P, I64, I, I, I, P, P, P, I, I, I, I, I, I, I, I, F32, P,
                                          I64, P, P]),
         "nemo_op_attention_window_form": (I, [I, I, I, I, I, I, I, I, I, I, I, I, I, P, P]),

@@ -188,3 +188,32 @@ def test_attention_window_splits_fit_the_device():
     assert window_form(max_k=32768, k_rows=32768, sms=8) == (0, 8)
     L = load_library()
     assert L.nemo_op_attention_window_form(3, 2, 128, 1, 1, 1, 1, 1, -1, -1, 0, 148, 16, None, None) == ERR_ARGS
+
+
+def w4_form(x_dtype, x_group, group, m, n, k, sms=148):
+    out = [ctypes.c_int() for _ in range(6)]
+    rc = load_library().nemo_op_w4_matvec_form(x_dtype, x_group, group, m, n, k, sms, *[ctypes.byref(v) for v in out])
+    assert rc == 0, load_library().nemo_last_error()
+    return dict(zip(("digits", "rows", "slices", "panels", "blocks", "shared"), [v.value for v in out]))
+
+
+def test_w4_matvec_forms():
+    """Up to two rows of 16-bit or e4m3 x, and i8 codes, as digits where there are many weight rows."""
+    assert w4_form(0, 0, 128, 1, 131072, 2048)["digits"] == 1
+    assert w4_form(1, 0, 128, 2, 50000, 1024)["digits"] == 1
+    assert w4_form(0, 0, 128, 3, 131072, 2048)["digits"] == 0
+    assert w4_form(4, 128, 128, 16, 131072, 2048)["digits"] == 1
+    assert w4_form(0, 0, 32, 16, 3, 12320)["panels"] > 1
+    L = load_library()
+    assert L.nemo_op_w4_matvec_form(2, 0, 128, 1, 1, 128, 148, None, None, None, None, None, None) == ERR_ARGS
+
+
+@pytest.mark.parametrize("x_dtype,x_group", [(0, 0), (3, 10 ** 9), (3, 32), (4, 64)])
+def test_w4_matvec_plans_two_blocks_an_sm_only_where_two_fit(x_dtype, x_group):
+    """An SM has 228 KB, of which every block takes 1 KB more than it asks for."""
+    for group in (32, 64, 128):
+        for m in range(1, 17):
+            for k in range(group, 12000, group):
+                form = w4_form(x_dtype, x_group, group, m, 200000, k)
+                if form["blocks"] > 148:
+                    assert 2 * (form["shared"] + 1024) <= 228 * 1024, (group, m, k, form)
