@@ -43,8 +43,8 @@ struct RowsCfg {
 };
 
 template <typename T, int D, int STAGES>
-__global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_constant__ AttnWindowArgs a, int splits,
-                                                                  int row_tiles) {
+__global__ void __launch_bounds__(kThreads) attention_rows_kernel(const __grid_constant__ AttnWindowArgs a,
+                                                                  int splits) {
   using C = RowsCfg<D, STAGES>;
   extern __shared__ __align__(1024) uint8_t smem[];
   dev::pdl_launch_dependents();
@@ -347,10 +347,9 @@ cudaError_t launch_rows(const AttnWindowArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     max_splits[dev] = blocks;
   }
-  const int64_t tiles = row_tiles(a);
   const int splits = attention_splits(a, max_splits[dev]);
-  const dim3 grid((unsigned)(tiles * splits), a.kv_heads, a.batch);
-  return launch_overlapped(kernel, grid, dim3(kThreads), C::kSmem, s, dim3(splits, 1), a, splits, (int)tiles);
+  const dim3 grid((unsigned)(row_tiles(a) * splits), a.kv_heads, a.batch);
+  return launch_overlapped(kernel, grid, dim3(kThreads), C::kSmem, s, dim3(splits, 1), a, splits);
 }
 
 }  // namespace
