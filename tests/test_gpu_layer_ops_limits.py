@@ -1,12 +1,15 @@
 """The layer operators of include/nemo_ops.h at the ends of their ranges: the smallest and largest values of a type,
 infinities in long prompts, long caches, and launch shapes between those of test_gpu_layer_ops.py."""
+import ctypes
 import math
 
+import numpy as np
 import pytest
 import torch
 
 import layer_ops_ref as ref
-from layer_ops_ref import BF16, F16, F32, TORCH
+from layer_ops_ref import BF16, E4M3, F16, F32, I8, TORCH
+from nemo_b200.runtime import check, load_library
 
 pytestmark = pytest.mark.gpu
 
@@ -16,6 +19,35 @@ def gen():
     g = torch.Generator(device="cuda")
     g.manual_seed(78)
     return g
+
+
+# --- rmsnorm_q8, rope_apply ------------------------------------------------------
+
+@pytest.mark.parametrize("dt,out", [(F16, I8), (BF16, E4M3)], ids=["f16_i8", "bf16_e4m3"])
+@pytest.mark.parametrize("rows,width", [(3, 264), (7, 512), (5, 765), (9, 768), (301, 1536), (151, 1100), (150, 20000)])
+def test_rmsnorm_q8_of_two_three_and_more_warps_a_row(gen, dt, out, rows, width):
+    """Blocks of several rows with a row missing at the end, and two or four vectors a thread."""
+    x, r = ((3 * torch.randn((rows, width), generator=gen, device="cuda")).to(TORCH[dt]) for _ in range(2))
+    w = 1 + 0.2 * torch.randn(width, generator=gen, device="cuda")
+    for group in (0, 32, 128):
+        ref.check_rmsnorm_q8(x, r, w, 1e-5, out, group, ref.rmsnorm_q8(x, r, w, 1e-5, out, group))
+
+
+@pytest.mark.parametrize("layout", [0, 1], ids=["pairs", "halves"])
+@pytest.mark.parametrize("pad", [0, 8, 1])
+@pytest.mark.parametrize("tokens", [1184, 1185, 2500])
+def test_rope_apply_of_many_tokens(gen, layout, pad, tokens):
+    """From eight tokens an SM on a block has fewer threads; rows that are 16 bytes apart or not."""
+    hq, hk, d, rotary = 6, 2, 64, 32
+    rows = torch.randn((tokens, (hq + hk) * d + pad), generator=gen, device="cuda").half()
+    ld = rows.stride(0)
+    q = torch.as_strided(rows, (tokens, hq, d), (ld, d, 1))
+    k = torch.as_strided(rows, (tokens, hk, d), (ld, d, 1), hq * d)
+    freq = torch.from_numpy(1e6 ** (-np.arange(0, rotary, 2) / rotary)).cuda()
+    pos = torch.randint(0, 40000, (tokens,), generator=gen, device="cuda", dtype=torch.int32)
+    qo, ko = ref.rope_apply(q, k, freq, 1.0, pos, rotary, layout)
+    ref.check_rope(q, freq, 1.0, pos, rotary, layout, qo)
+    ref.check_rope(k, freq, 1.0, pos, rotary, layout, ko)
 
 
 # --- w4_matvec -------------------------------------------------------------------
@@ -176,3 +208,33 @@ def test_attention_window_many_small_weights(gen, batch, q_len, nk, heads, warps
     error = float(((got - want) / want).abs().max())
     print(f"relative error {error:.2e}")
     assert error <= 2 * 2.0 ** -11 + 2.0 ** -15 + nk / warps / 16 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("qs,ks", [([512, 1, 1, 1], [512, 3000, 1, 777]), ([1, 1, 2048, 0, 1], [64, 900, 2048, 5, 4000])])
+def test_attention_window_of_a_prompt_among_single_tokens(gen, qs, ks):
+    hq, hk, d = 24, 8, 128
+    q = torch.randn((sum(qs), hq, d), generator=gen, device="cuda").half()
+    k, v = (torch.randn((sum(ks), hk, d), generator=gen, device="cuda").half() for _ in range(2))
+    q_off, start = [0] + np.cumsum(qs).tolist(), [0] + np.cumsum(ks).tolist()[:-1]
+    got = ref.attention(q, k, v, q_off, start, ks, 1023, 0, 4)
+    ref.check_attention(q, k, v, q_off, start, ks, 1023, 0, 4, got)
+
+
+# --- memory ----------------------------------------------------------------------
+
+def test_managed_memory_is_served(gen):
+    rt = ctypes.CDLL("libcudart.so.12")
+    x, w = torch.randn((4, 256), generator=gen, device="cuda").half(), torch.ones(256, device="cuda")
+    _, want, scales = ref.rmsnorm_q8(x, None, w, 1e-5, I8, 0)
+    p = ctypes.c_void_p()
+    assert rt.cudaMallocManaged(ctypes.byref(p), ctypes.c_size_t(4 * 256), ctypes.c_uint(1)) == 0
+    try:
+        sc = torch.zeros((4, 1), device="cuda")
+        check(load_library().nemo_op_rmsnorm_q8(F16, x.data_ptr(), 256, None, 0, w.data_ptr(), 4, 256, 1e-5, None, 0, I8,
+                                                0, p.value, 256, sc.data_ptr(), ref.stream()))
+        torch.cuda.synchronize()
+        got = np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_int8)), (4, 256)).copy()
+    finally:
+        torch.cuda.synchronize()
+        assert rt.cudaFree(p) == 0
+    assert np.array_equal(got, want.cpu().numpy()) and torch.equal(sc, scales)
