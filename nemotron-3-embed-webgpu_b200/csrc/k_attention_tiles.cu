@@ -715,17 +715,20 @@ int64_t visible_keys(const AttnWindowArgs& a, int rows) {
 }
 
 // Prompts and documents run on the 128-row tiles, few queries on 16-row ones,
-// whichever a model of both calls faster. Measured with 24 + 8 heads of 128, us:
-// the 16-row kernel takes 6 + (row tiles x keys of all requests) / 13000, this one
-// 5 + 0.85 a step of 64 keys and round of pairs over the SMs. 16 x 8 queries on
-// 1500 keys 31 against 51, 16 x 32 88 against 51; 1 x 64 on 16384 111 against
-// 222, 1 x 128 204 against 224.
+// whichever a model of both calls faster: 4 us + (row tiles x keys of all requests)
+// over a rate for the 16-row kernel, 5 us + a time for each step of 64 keys and
+// round of pairs over the SMs for this one. Measured with 24 + 8 heads, us (16-row
+// against this), queries on keys of 128, then of 64 columns: 16 x 8 on 1500 32 / 53
+// and 34 / 49, 16 x 32 89 / 53 and 55 / 50, 4 x 64 on 4096 112 / 65 and 71 / 61,
+// 1 x 64 on 16384 112 / 238 and 74 / 223, 1 x 128 206 / 239 and 135 / 224, 1 x 256
+// 394 / 239 and 259 / 226; 8 x 2 on 56 of 64 columns 4.0 / 6.6.
 bool attention_on_tiles(const AttnWindowArgs& a) {
   const int group = a.q_heads / a.kv_heads;
   const double row_tiles = (double)(((int64_t)a.max_q * group + 15) / 16) * a.kv_heads * a.batch;
   const double pairs = (double)((((int64_t)a.max_q + kRows - 1) / kRows * group + 1) / 2) * a.kv_heads * a.batch;
-  const double few = 6 + row_tiles * visible_keys(a, 16) / 13000;
-  const double many = 5 + ceil(pairs / a.sms) * visible_keys(a, kRows + kKeys) * (0.85 / kKeys);
+  const double rate = a.head_dim == 64 ? 23500 : 15000, step = a.head_dim == 64 ? 0.86 : 0.92;
+  const double few = 4 + row_tiles * visible_keys(a, 16) / rate;
+  const double many = 5 + ceil(pairs / a.sms) * visible_keys(a, kRows + kKeys) * (step / kKeys);
   return few > many && a.k_rows > 0;
 }
 

@@ -220,6 +220,31 @@ def test_attention_window_of_a_prompt_among_single_tokens(gen, qs, ks):
     ref.check_attention(q, k, v, q_off, start, ks, 1023, 0, 4, got)
 
 
+def window_form(hq, hk, d, batch, q_rows, k_rows, max_q, max_k, left, right, sinks):
+    tiles, splits = ctypes.c_int(), ctypes.c_int()
+    check(load_library().nemo_op_attention_window_form(hq, hk, d, batch, q_rows, k_rows, max_q, max_k, left, right, sinks,
+                                                       148, 16, ctypes.byref(tiles), ctypes.byref(splits)))
+    return tiles.value, splits.value
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [(-1, -1, 0), (-1, 0, 0), (70, 0, 3), (40, 130, 65), (100, 33, 0)],
+                         ids=lambda w: "l%d_r%d_s%d" % w)
+def test_attention_window_around_the_edges_of_the_tiles(gen, dt, d, window):
+    """Lengths beside multiples of the 128 queries and 64 keys of a tile, one to three heads a kv head, each on the
+    128-query tiles."""
+    for hq, hk in ((24, 8), (8, 8)):
+        qs = [127, 1, 128, 129, 0, 255, 257, 64, 320, 700, 700, 700]
+        ks = [127, 64, 129, 65, 9, 256, 511, 700, 321, 700, 701, 763]
+        q = torch.randn((sum(qs), hq, d), generator=gen, device="cuda").to(TORCH[dt])
+        k, v = (torch.randn((sum(ks), hk, d), generator=gen, device="cuda").to(TORCH[dt]) for _ in range(2))
+        assert window_form(hq, hk, d, len(qs), sum(qs), sum(ks), max(qs), max(ks), *window)[0] == 1
+        q_off, start = [0] + np.cumsum(qs).tolist(), [0] + np.cumsum(ks).tolist()[:-1]
+        got = ref.attention(q, k, v, q_off, start, ks, *window)
+        ref.check_attention(q, k, v, q_off, start, ks, *window, got)
+
+
 # --- memory ----------------------------------------------------------------------
 
 def test_managed_memory_is_served(gen):

@@ -217,3 +217,15 @@ def test_w4_matvec_plans_two_blocks_an_sm_only_where_two_fit(x_dtype, x_group):
                 form = w4_form(x_dtype, x_group, group, m, 200000, k)
                 if form["blocks"] > 148:
                     assert 2 * (form["shared"] + 1024) <= 228 * 1024, (group, m, k, form)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("batch,q_len,k_len,tiles", [
+    (16, 8, 1500, 0), (16, 32, 1500, 1), (4, 64, 4096, 1), (1, 64, 16384, 0), (1, 128, 16384, 0), (1, 256, 16384, 1),
+    (8, 2, 56, 0)])
+def test_attention_window_takes_the_form_that_measures_faster(head_dim, batch, q_len, k_len, tiles):
+    """128 queries on 16384 keys: 206 us in 16-row tiles and 239 in 128-query ones (128 columns), 135 and 224 (64); eight
+    requests of 2 on 56 keys 4.0 and 6.6."""
+    form = window_form(head_dim=head_dim, batch=batch, q_rows=batch * q_len, max_q=q_len, k_rows=batch * k_len,
+                       max_k=k_len)
+    assert form[0] == tiles
