@@ -162,7 +162,9 @@ int nemo_op_qmatmul_image_decode(int fmt, const void* d_image, int n, int k, voi
  * [rows x ceil(width / group)]. d_sum is NULL exactly when d_residual is; it
  * may be d_x or d_residual themselves (with the same ld). A group whose top is
  * at most 1e-30 has codes 0; one that holds an infinity or a NaN has codes 0
- * and a NaN scale. width <= 32768. Rows of 16-byte multiples with 16-byte
+ * and a NaN scale. mean(s^2) is an f32 sum too: values whose squares leave its
+ * range (above 1e19 / sqrt(width); with eps 0, below 1e-19) have no useful
+ * scale. width <= 32768. Rows of 16-byte multiples with 16-byte
  * aligned buffers (8-byte for d_q) are read and written as vectors; others
  * work, slower. */
 int nemo_op_rmsnorm_q8(int dtype, const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, const void* d_w,
@@ -223,7 +225,8 @@ int nemo_rope_inv_freq(int scaling, double theta, int rotary_dim, double factor,
  * row (as nemo_op_rmsnorm_q8 writes them, where group 0 is x_group >= k);
  * 16-bit x takes NULL. y is F16, BF16 or F32. Sums are f32 or finer and y is
  * rounded once; 16-bit elements of x below 2^-19 of the largest of their 32 to
- * 128 neighbours may be rounded to 2^-30 of it. An infinity or NaN in a row of
+ * 128 neighbours may be rounded to 2^-30 of it. A sum of x * (q - zero) over one
+ * group must stay within f32 (it does for |x| up to 2^116). An infinity or NaN in a row of
  * x makes its row of y infinite or NaN. m > 16 is refused: more rows take a call
  * for each 16 of them, which reads the weights each time (no other entry takes
  * this format). n and k are at most 2^30. d_x and ldx need the alignment of one
@@ -252,7 +255,9 @@ int nemo_op_w4_matvec_form(int x_dtype, int x_group, int group, int m, int n, in
  * no key, or whose scores are all -infinity, gets zeros. Scores are q . k *
  * scale with an f32 softmax, weights are rounded to dtype for the product with
  * v, which sums in f32. Infinities and NaN in keys or values that a query does
- * not see do not reach its row. dtype F16 or BF16; head_dim 64 or 128; q_heads
+ * not see do not reach its row; a NaN that it sees makes its columns of the row
+ * NaN, or the whole row if it is in a score (as does a score of +infinity).
+ * Finite values never give an infinite result. dtype F16 or BF16; head_dim 64 or 128; q_heads
  * a multiple of kv_heads; heads follow one another within a row; batch and
  * heads at most 65535; buffers 16-byte aligned, leading dimensions multiples
  * of 8. q_rows, k_rows: rows of the buffers, in which the offsets have to lie.

@@ -13,24 +13,26 @@
 //   O += P . V    (tcgen05, P from tensor memory, O stays there)
 // Each unit has two S tiles in tensor memory (2 x 64 columns beside 128 of O;
 // two units fill the 512): the products of the next key tile are ready when a
-// softmax ends, so neither side waits for the other's latency. (Tiles of 128
-// keys with one S of 128 columns: 347 us where these take 180.)
+// softmax ends, so neither side waits for the other's latency. (When they came in,
+// 180 us for the 8,192 tokens below, 347 with tiles of 128 keys and one S of 128
+// columns.)
 //
 // The window: a block's key tiles start at its first visible key, the sinks in
 // front of it have tiles of their own behind the window's (the running maximum
-// that a window leaves rarely moves again: 106 us at sixteen requests of 1 to
-// 1,500 tokens, 24 heads of 128, window 128 + 128 and one sink, where sinks in
-// front take 109), and each product covers only the 32-key chunks that some
+// that a window leaves rarely moves again: sinks in front took 3 % more for
+// sixteen requests of 1 to 1,500 tokens, 24 heads of 128, window 128 + 128 and one
+// sink), and each product covers only the 32-key chunks that some
 // query of the unit sees. Within a tile each warp leaves out the chunks that
 // none of its 32 rows sees and masks only those that some of them do not see
 // whole.
 //
 // Bound: both the tensor cores and the exponential unit need 512 cycles per
 // 128 x 64 tile at head size 128. Measured: a prompt of 8,192 tokens, heads as
-// above, causal with 2,048 keys a query 166 us (1.09 PFLOP/s of the visible
-// pairs); the sixteen above 102 us, where half of the tiles are masked ones and
-// each pair of units has six or seven. Of those 102 us the masks and maxima are
-// 12, the output 16 and the sink 12.
+// above, causal with 2,048 keys a query 166 to 177 us on different cards (1.02 to
+// 1.09 PFLOP/s of the visible pairs) in a row of launches, 201 for one launch
+// between two events; the sixteen above 102 to 104 us, where half of the tiles are
+// masked ones and each pair of units has six or seven: the masks and maxima are
+// about 12 us of it, the output 16 and the sink 12.
 //
 // Warps (384 threads, persistent, one block per SM): 0 copies Q, K and V (TMA),
 // 1 and 2 issue the units' products (a warp each: the tensor pipe takes one
@@ -156,7 +158,7 @@ struct Items {
   }
   // The block's i-th item: every other round of the blocks runs backwards, so
   // that the blocks with the longest pairs of one round get the shortest of the
-  // next (8192 causal queries: 178 us without, 167).
+  // next (8192 causal queries when it came in: 178 us without, 167 with it).
   __device__ __forceinline__ int nth(int i) const {
     return i * (int)gridDim.x + (i & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
   }
@@ -495,7 +497,7 @@ __global__ void __launch_bounds__(384, 1)
         dev::tc_wait_ld();
         // A tile that every row sees takes its weights against the reference that
         // it has straight away. They stand if every row's sum is at most 2^15 (with 2^8 as
-        // the limit more tiles go twice: 106 us for the 102 above): then no
+        // the limit more tiles go twice: 106 us for 102): then no
         // weight is above that either, inside the 16-bit types, and O needs no
         // rescaling. Otherwise the tile's own maximum is found, the reference
         // moves and the weights are taken again. (A NaN fails the comparison.)

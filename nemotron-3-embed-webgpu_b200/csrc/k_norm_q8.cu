@@ -11,7 +11,7 @@
 // the writes. wpr warps share a row, NV 8-column vectors per thread. With a
 // dozen scalar operations per element the kernel was bound by instructions (89
 // us at 24000 x 2048, bf16 to e4m3); packed f32 pairs, maxima of three and one
-// division per group brought it to 57, 92 % of the copy rate.
+// division per group brought it to 57, 93 % of the copy rate.
 #include "layer_ops.cuh"
 
 namespace nemo {

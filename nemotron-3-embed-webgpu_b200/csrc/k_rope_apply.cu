@@ -1,5 +1,5 @@
 // Rotary embedding for any head size, rotated part and pair layout
-// (nemo_op_rope_apply), and the host frequencies of scaled contexts.
+// (nemo_op_rope_apply; its frequencies come from nemo_rope_inv_freq, layer_ops.cu).
 //
 // The angle of position p and pair i is p * f_i; only its fraction of a turn
 // matters. p * f_i / 2pi is formed in f64 (a position of 2^31 keeps the

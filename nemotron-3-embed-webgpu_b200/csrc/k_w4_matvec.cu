@@ -35,17 +35,17 @@
 // summed over warps; more where there are few rows. Panels (of the columns
 // whose x fits shared memory) of a row tile are blocks of one cluster, summed in
 // rank order through distributed shared memory. (Chunks of all the block's tiles
-// in one stream, an eighth for each warp, balance better, 28.9 us where this
-// took 31.0, but the sums of tiles that warps share cost 0.3 us in small calls and
-// twice the time where a row takes several panels.)
+// in one stream, an eighth for each warp, balanced better, 28.9 us against 31.0
+// when the two were compared, but the sums of tiles that warps share cost 0.3 us in
+// small calls and twice the time where a row takes several panels.)
 //
 // Bound: at 6.5 TB/s an SM gets 4 KB of weights (32 rows x 256 columns) in 180
 // cycles, in which its schedulers issue 720 instructions; the floating-point form
 // takes some 750 for them, digits about 450. One row of bf16 x against 131072 x
-// 2048: 29.0 us with digits, 4.8 TB/s (37.7 without); 512 tiles are 1.7 rounds of
-// 296 blocks, and the last round is the most of what is missing. (16-row tiles
-// 61, a fixed split of every tile over the 8 warps 51, 64 with the scales read in
-// line and two logic operations a nibble pair, all without digits.) One row
+// 2048: 29.4 us with digits, 4.7 TB/s (37.7 without); 512 tiles are 1.7 rounds of
+// 296 blocks, and the last round is the most of what is missing. (Earlier
+// versions without digits: 16-row tiles 61, a fixed split of every tile over the 8
+// warps 51, scales read in line and two logic operations a nibble pair 64.) One row
 // against 5120 x 2048: 4.9 us.
 #include <type_traits>
 
@@ -772,9 +772,9 @@ bool plan_w4(const W4Args& a, bool xg, int seg, W4Plan& best) {
   // for each eight elements a thread prepares. One f16 row, group 128, us with
   // digits and without: 131072 x 2048 29 / 38, 5120 x 2048 4.8 / 5.0, 2048 x 6144
   // 7.4 / 6.6; group 64, 6144 x 6144: 14.8 / 10.7; sixteen i8 rows, 131072 x 2048
-  // 59 / 83, 5120 x 2048 11.4 / 11.0. Digits take four columns a row of x, so
-  // they are for two rows at most (four rows against 131072 x 2048: 50 us, 42
-  // without) and for i8, where they are one.
+  // 60 / 83, 5120 x 2048 11.4 / 11.0. Digits take four columns a row of x, so
+  // they are for two rows at most (four rows against 131072 x 2048 took 50 us
+  // with them; 39 without) and for i8, where they are one.
   const double digit_chunk = seg == 128 ? 0.8 : seg == 64 ? 1.0 : 1.2;
   for (int digits = 0; digits < (a.x_dtype == kDtI8 || a.m <= 2 ? 2 : 1); ++digits) {
     W4Plan p = {};
