@@ -74,13 +74,17 @@ def test_w4_matvec_of_the_smallest_bf16_values(gen, shift, m, n):
 # --- attention_window ------------------------------------------------------------
 
 def milliseconds(call):
+    """The shortest of five, so that a pause of the host between the events does not count."""
     call()
-    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-    a.record()
-    call()
-    b.record()
-    torch.cuda.synchronize()
-    return a.elapsed_time(b)
+    times = []
+    for _ in range(5):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
 
 
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
